@@ -227,11 +227,14 @@ def _act(v, kind):
 
 def _quantised(st):
     # In 64 bits: a value next to the border of two steps falls to either side
-    # with the last bits of its quotient.
+    # with the last bits of its quotient.  A tensor divides (a Python number
+    # would multiply by its rounded reciprocal): a value on the border then
+    # goes to the even code.
     x = st["x"].double()
     if st["case"]["op"] != "linear":
         x = x * st["norm_w"] / torch.sqrt((x * x).mean(dim=1, keepdim=True) + st["eps"])
-    scale = x.abs().amax(dim=1, keepdim=True) / 127.0
+    amax = x.abs().amax(dim=1, keepdim=True)
+    scale = amax / torch.full_like(amax, 127.0)
     return (x / scale).round().float(), scale.float()
 
 
@@ -296,7 +299,8 @@ def exact(case, seed):
     if "norm_w" in st:
         rms = torch.linalg.vector_norm(x, dim=1) / math.sqrt(case["K"])
         x = st["norm_w"].to(d) * (x / torch.sqrt(rms ** 2 + st["eps"])[:, None])
-    step = x.abs().max(dim=1).values / 127
+    largest = x.abs().max(dim=1).values
+    step = torch.true_divide(largest, torch.tensor(127.0, dtype=d, device=largest.device))
     codes = torch.round(x / step[:, None])
 
     def proj(w, scale):
