@@ -11,6 +11,7 @@
 #include "ffwd_b200.h"
 #include "attention.cuh"
 #include "gemm.cuh"
+#include "host_util.h"
 #include "loader.h"
 #include "ptx.cuh"
 #include "late.cuh"
@@ -33,11 +34,13 @@
 #include <vector>
 
 namespace fb {
+
+std::atomic<long long> g_launches{0};
+
 namespace {
 
 // ------------------------------------------------------------------ globals
 
-std::atomic<long long> g_launches{0};
 int g_gemm_mode = 0;         // 0 f32, 1 tf32, 2 bf16, 3 16f (reference default: f32)
 int g_weight_override = -1;  // -1 file dtype, 0 f32, 1 bf16, 2 f16
 std::vector<int> g_devices;
@@ -50,6 +53,8 @@ thread_local std::string t_err;
 std::atomic<int> g_inject_shard{-1};
 std::atomic<int> g_inject_alloc{0};
 
+}  // namespace
+
 void fail(const char *fmt, ...) {
     char buf[512];
     va_list ap;
@@ -60,21 +65,9 @@ void fail(const char *fmt, ...) {
     fprintf(stderr, "ffwd_b200: %s\n", buf);
 }
 
-#define CK(expr)                                                                              \
-    do {                                                                                      \
-        cudaError_t _e = (cudaError_t)(expr);                                                 \
-        if (_e != cudaSuccess) {                                                              \
-            fail("%s failed: %s (%s:%d)", #expr, cudaGetErrorString(_e), __FILE__, __LINE__); \
-            return -1;                                                                        \
-        }                                                                                     \
-    } while (0)
+void clear_error() { t_err.clear(); }
 
-// Kernel launch wrappers return a cudaError_t value; count every launch.
-#define LAUNCH(expr)             \
-    do {                         \
-        g_launches.fetch_add(1); \
-        CK(expr);                \
-    } while (0)
+namespace {
 
 // ------------------------------------------------------------------ tensor maps
 
@@ -97,9 +90,11 @@ EncodeTiledFn encode_fn() {
     return fn;
 }
 
-// 2-D row-major matrix [rows, cols] of `esz`-byte elements; box = box_rows x box_cols.
-int make_map_dt(CUtensorMap *m, const void *ptr, uint64_t rows, uint64_t cols, uint32_t box_rows,
-                uint32_t box_cols, CUtensorMapSwizzle sw, CUtensorMapDataType dt, int esz) {
+}  // namespace
+
+int make_map_ld(CUtensorMap *m, const void *ptr, uint64_t rows, uint64_t cols, uint64_t ld,
+                uint32_t box_rows, uint32_t box_cols, CUtensorMapSwizzle sw,
+                CUtensorMapDataType dt, int esz) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) {
         fail("cuTensorMapEncodeTiled unavailable");
@@ -107,7 +102,7 @@ int make_map_dt(CUtensorMap *m, const void *ptr, uint64_t rows, uint64_t cols, u
     }
     if (rows == 0) rows = 1;
     const cuuint64_t dims[2] = {cols, rows};
-    const cuuint64_t strides[1] = {cols * (uint64_t)esz};
+    const cuuint64_t strides[1] = {ld * (uint64_t)esz};
     const cuuint32_t box[2] = {box_cols, box_rows};
     const cuuint32_t estr[2] = {1, 1};
     CUresult r = fn(m, dt, 2, const_cast<void *>(ptr), dims, strides, box, estr,
@@ -119,6 +114,14 @@ int make_map_dt(CUtensorMap *m, const void *ptr, uint64_t rows, uint64_t cols, u
         return -1;
     }
     return 0;
+}
+
+namespace {
+
+// 2-D row-major matrix [rows, cols] of `esz`-byte elements; box = box_rows x box_cols.
+int make_map_dt(CUtensorMap *m, const void *ptr, uint64_t rows, uint64_t cols, uint32_t box_rows,
+                uint32_t box_cols, CUtensorMapSwizzle sw, CUtensorMapDataType dt, int esz) {
+    return make_map_ld(m, ptr, rows, cols, cols, box_rows, box_cols, sw, dt, esz);
 }
 
 // 2-D 16-bit row-major matrix [rows, cols]; box = box_rows x box_cols.  Also used

@@ -23,6 +23,7 @@ enum DevError : int {
     kErrBadNorm = 2,       // zero / non-finite embedding norm (reference: vec.c:13-14)
     kErrBadTokenId = 3,    // token id outside [0, vocab) (reference: forward.c:224-228)
     kErrSmemAlign = 4,     // dynamic shared memory window not 1024-byte aligned
+    kErrBadPosition = 5,   // position outside the rotary tables
 };
 
 // ~2 s: far above any legitimate wait inside one launch.
@@ -394,6 +395,20 @@ __device__ __forceinline__ float2 add_f32x2(float2 a, float2 b) {
 // Named barrier `id` (1..15) over `count` threads.
 __device__ __forceinline__ void named_bar(int id, int count) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
+}
+
+// The same, returning whether `pred` holds for all of the threads.
+__device__ __forceinline__ bool named_bar_and(int id, int count, bool pred) {
+    uint32_t out;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %3, 0;\n\t"
+        "bar.red.and.pred q, %1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(out)
+        : "r"(id), "r"(count), "r"((uint32_t)pred)
+        : "memory");
+    return out != 0;
 }
 
 // ----------------------------------------------------------------- descriptors

@@ -47,6 +47,17 @@ class ffwd_config_t(ctypes.Structure):
             "append_terminal_token")]
 
 
+class ffwd_b200_i8_mat_t(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+                ("rows", ctypes.c_int), ("cols", ctypes.c_int), ("ld", ctypes.c_longlong)]
+
+
+class ffwd_b200_i8_heads_t(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("n_heads", "n_kv_heads", "head_dim", "n_pos")] + [
+        (n, ctypes.c_void_p) for n in ("pos", "cos", "sin", "q_norm", "k_norm")] + [
+        ("eps", ctypes.c_float)]
+
+
 class ffwd_rerank_input_t(ctypes.Structure):
     _fields_ = [("query_ids", ctypes.POINTER(ctypes.c_int)), ("query_n_tokens", ctypes.c_int),
                 ("query_n_keep", ctypes.c_int),
@@ -106,6 +117,22 @@ ABI = {
                                            ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     "ffwd_b200_gemm_tf32": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                            ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "ffwd_b200_quantize_i8": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_float,
+        ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_int, ctypes.c_int,
+        ctypes.c_void_p]),
+    "ffwd_b200_gemm_i8": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_int,
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_int, ctypes.c_int,
+        ctypes.c_void_p, ctypes.c_void_p]),
+    "ffwd_b200_gated_i8": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
+        ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_int,
+        ctypes.c_void_p, ctypes.c_void_p]),
+    "ffwd_b200_qkv_i8": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
+        ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p,
+        ctypes.c_void_p]),
     "ffwd_b200_encode_batch_as": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
                                                  ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                                  ctypes.c_void_p]),
@@ -443,6 +470,65 @@ def gemm_tf32(x_ptr, w_ptr, y_ptr, M, N, K, bn=256):
     rc = lib().ffwd_b200_gemm_tf32(x_ptr, w_ptr, y_ptr, M, N, K, bn)
     if rc != 0:
         raise FfwdError(f"gemm failed: {last_error()}")
+
+
+# 8-bit integer projections (see include/ffwd_b200.h).  Pointers are device
+# addresses; strides are in elements; `stream` is a cudaStream_t address (0: the
+# default stream).
+I8_TYPES = {"f32": 0, "bf16": 1, "f16": 2}
+I8_ACTS = {"none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3}
+
+
+def i8_mat(q_ptr, scale_ptr, rows, cols, ld, bias_ptr=None) -> ffwd_b200_i8_mat_t:
+    """Descriptor of int8 weights [rows, cols] with a scale (and bias) per row."""
+    return ffwd_b200_i8_mat_t(q_ptr, scale_ptr, bias_ptr, rows, cols, ld)
+
+
+def i8_heads(n_heads, n_kv_heads, head_dim, pos_ptr, cos_ptr, sin_ptr, n_pos, q_norm_ptr=None,
+             k_norm_ptr=None, eps=0.0) -> ffwd_b200_i8_heads_t:
+    """Heads of a fused QKV projection: positions, rotary tables, head norms."""
+    return ffwd_b200_i8_heads_t(n_heads, n_kv_heads, head_dim, n_pos, pos_ptr, cos_ptr, sin_ptr,
+                                q_norm_ptr, k_norm_ptr, eps)
+
+
+def _i8_code(table, name):
+    if name not in table:
+        raise FfwdError(f"{name!r} is not one of {', '.join(table)}")
+    return table[name]
+
+
+def _i8_check(rc, what):
+    if rc != 0:
+        raise FfwdError(f"{what} failed: {last_error()}")
+
+
+def quantize_i8(x_ptr, dtype, ldx, q_ptr, ldq, scale_ptr, M, K, norm_ptr=None, eps=0.0, stream=0):
+    """Rows to int8 with a scale each, optionally after an RMSNorm with weights
+    at norm_ptr."""
+    _i8_check(lib().ffwd_b200_quantize_i8(x_ptr, _i8_code(I8_TYPES, dtype), ldx, norm_ptr, eps, q_ptr, ldq,
+                                          scale_ptr, M, K, stream), "quantize_i8")
+
+
+def gemm_i8(w, x_ptr, ldx, xs_ptr, M, y_ptr, dtype, ldy, act="none", accumulate=False,
+            err_ptr=None, stream=0):
+    """y = act(x w^T) (accumulate: y +=) of quantised rows with weights `w` (i8_mat)."""
+    _i8_check(lib().ffwd_b200_gemm_i8(ctypes.byref(w), x_ptr, ldx, xs_ptr, M, y_ptr,
+                                      _i8_code(I8_TYPES, dtype), ldy, _i8_code(I8_ACTS, act), int(accumulate),
+                                      err_ptr, stream), "gemm_i8")
+
+
+def gated_i8(gate, up, x_ptr, ldx, xs_ptr, M, h_ptr, dtype, ldh, act="silu", err_ptr=None,
+             stream=0):
+    """h = act(x gate^T) * (x up^T) of quantised rows."""
+    _i8_check(lib().ffwd_b200_gated_i8(ctypes.byref(gate), ctypes.byref(up), x_ptr, ldx, xs_ptr, M,
+                                       h_ptr, _i8_code(I8_TYPES, dtype), ldh, _i8_code(I8_ACTS, act), err_ptr,
+                                       stream), "gated_i8")
+
+
+def qkv_i8(w, heads, x_ptr, ldx, xs_ptr, M, out_ptr, dtype, ldo, err_ptr=None, stream=0):
+    """Fused QKV projection of quantised rows, head norms and rotation included."""
+    _i8_check(lib().ffwd_b200_qkv_i8(ctypes.byref(w), ctypes.byref(heads), x_ptr, ldx, xs_ptr, M,
+                                     out_ptr, _i8_code(I8_TYPES, dtype), ldo, err_ptr, stream), "qkv_i8")
 
 
 class FfwdApi:

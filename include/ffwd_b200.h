@@ -329,6 +329,89 @@ FFWD_B200_API int ffwd_b200_gemm_bf16(const void *x, const void *x_lo, const voi
 FFWD_B200_API int ffwd_b200_gemm_tf32(const float *x, const float *w, float *y, int M, int N, int K,
                                       int bn);
 
+/* ---- 8-bit integer projections ----------------------------------------------
+ *
+ * No counterpart in the reference.  Rows are quantised to int8 with one scale
+ * each, weights hold one scale per output channel, and the products are summed
+ * exactly in 32-bit integers:
+ *
+ *   q[m, k] = rint(x[m, k] / s[m]), s[m] = max_k |x[m, k]| / 127
+ *   y[m, n] = (sum_k q[m, k] w.q[n, k]) * s[m] * w.scale[n] + w.bias[n]
+ *
+ * All pointers are device memory of the current device (other memory is
+ * refused), except the descriptors, which are read on the host during the call.
+ * Work is enqueued on `stream` (a cudaStream_t of the current device; NULL is
+ * the default stream); nothing is allocated, kept or synchronised, so the calls
+ * can be captured into CUDA graphs.  Outputs must not overlap inputs.  M = 0
+ * is an empty call.  `err` is an int in device memory, zeroed by the caller,
+ * or NULL: a kernel that fails records a nonzero code there (1: a device wait
+ * ran out, 5: a position outside the rotary tables). */
+enum {
+    FFWD_B200_F32 = 0,
+    FFWD_B200_BF16 = 1,
+    FFWD_B200_F16 = 2
+};
+
+enum {
+    FFWD_B200_ACT_NONE = 0,
+    FFWD_B200_ACT_SILU = 1,
+    FFWD_B200_ACT_GELU_ERF = 2,
+    FFWD_B200_ACT_GELU_TANH = 3
+};
+
+/* int8 weights [rows, cols] (rows: output channels): 16-byte aligned, row
+ * stride ld a multiple of 16, cols <= 131071.  The bytes between cols and ld
+ * may hold anything; up to the next multiple of 16 they may be read (the last
+ * row's too), as in quantised rows x below.  bias may be NULL. */
+typedef struct {
+    const int8_t *q;
+    const float *scale; /* [rows] */
+    const float *bias;  /* [rows] or NULL */
+    int rows, cols;
+    long long ld;
+} ffwd_b200_i8_mat_t;
+
+/* Heads of a fused query / key / value projection (rows: n_heads query heads,
+ * n_kv_heads key heads, n_kv_heads value heads, head_dim 64 or 128 each). */
+typedef struct {
+    int n_heads, n_kv_heads, head_dim, n_pos;
+    const int *pos;      /* [M] position of each row, in [0, n_pos) */
+    const float *cos;    /* [n_pos, head_dim / 2], 16-byte aligned */
+    const float *sin;
+    const float *q_norm; /* [head_dim], 16-byte aligned, or NULL: no norm */
+    const float *k_norm;
+    float eps;
+} ffwd_b200_i8_heads_t;
+
+/* x [M, K] of `type` (row stride ldx elements) -> q int8 [M, K] (16-byte
+ * aligned, row stride ldq a multiple of 16; bytes past K are left alone) and
+ * scale [M].  With `norm` [K], of x * norm / sqrt(mean(x^2) + eps) instead.
+ * A row of zeros gets scale 0; a row with a value (or, with `norm`, a sum of
+ * squares) that is not finite gets scale NaN and zeros.  Also quantises
+ * weights: a row per output channel. */
+FFWD_B200_API int ffwd_b200_quantize_i8(const void *x, int type, long long ldx, const float *norm,
+                                        float eps, int8_t *q, long long ldq, float *scale, int M,
+                                        int K, void *stream);
+/* y [M, w.rows] = act(x w^T) of `type` (row stride ldy elements); accumulate
+ * (f32 only): y += instead.  x, xs: quantised rows and their scales. */
+FFWD_B200_API int ffwd_b200_gemm_i8(const ffwd_b200_i8_mat_t *w, const int8_t *x, long long ldx,
+                                    const float *xs, int M, void *y, int type, long long ldy,
+                                    int act, int accumulate, int *err, void *stream);
+/* Gated feed-forward: h [M, gate.rows] = act(x gate^T) * (x up^T), both
+ * projections, the activation and the product in one kernel. */
+FFWD_B200_API int ffwd_b200_gated_i8(const ffwd_b200_i8_mat_t *gate, const ffwd_b200_i8_mat_t *up,
+                                     const int8_t *x, long long ldx, const float *xs, int M,
+                                     void *h, int type, long long ldh, int act, int *err,
+                                     void *stream);
+/* Fused query / key / value projection: out [M, w.rows] = x w^T, each query and
+ * key head then divided by its RMS and weighted (where q_norm / k_norm is
+ * given) and rotated to its row's position (element i with element i +
+ * head_dim / 2), in the same kernel.  A row whose position is outside [0,
+ * n_pos) gets NaN in its query and key heads and code 5 in *err. */
+FFWD_B200_API int ffwd_b200_qkv_i8(const ffwd_b200_i8_mat_t *w, const ffwd_b200_i8_heads_t *heads,
+                                   const int8_t *x, long long ldx, const float *xs, int M,
+                                   void *out, int type, long long ldo, int *err, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
