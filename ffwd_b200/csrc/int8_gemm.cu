@@ -28,18 +28,26 @@ constexpr int BK = 128;       // bytes of K per stage
 constexpr int kGroups = 2;    // epilogue warpgroups
 constexpr int kThreads = 64 + 128 * kGroups;
 constexpr int A_BYTES = BM * BK;
-constexpr int CHUNK = 8192;   // 128 rows x 64 bytes of output
+constexpr int CHUNK = 2048;   // 32 rows x 64 bytes of output
 constexpr uint32_t kPeerMask = 0xFEFFFFFFu;  // clears the CTA-rank bit: leader's copy
 
-template <int BN>
+// Shared memory.  The head form keeps the rotary rows of the CTA's 128 rows
+// (cos and sin, f32, each row padded by 16 bytes so that 32 lanes reading 16
+// bytes of a row each meet no bank twice) and writes its heads straight from
+// registers; the others stage 2 KB of output per epilogue warp, twice.
+template <int BN, int EPI, int HD>
 struct Cfg {
+    static constexpr bool HEADS = EPI == kI8Heads;
     static constexpr int B_BYTES = (BN / 2) * BK;  // this CTA's half of the weight rows
     static constexpr int STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = BN == 256 ? 5 : BN == 128 ? 7 : 8;
+    static constexpr int STAGES = HEADS ? (BN == 256 ? 4 : 5) : BN == 256 ? 5 : BN == 128 ? 7 : 8;
     static constexpr int OFF_STAGING = STAGES * STAGE;
-    static constexpr int OFF_COLS = OFF_STAGING + kGroups * 2 * CHUNK;
-    // Per warpgroup: the tile's scales and biases.
-    static constexpr int SMEM = OFF_COLS + kGroups * 2 * BN * 4 + 1024;
+    static constexpr int ROPE_LD = HD + 4;  // floats
+    static constexpr int STAGING = HEADS ? BM * ROPE_LD * 4 : 4 * kGroups * 2 * CHUNK;
+    // Per warpgroup, twice: the tile's scales and biases.
+    static constexpr int OFF_COLS = OFF_STAGING + STAGING;
+    static constexpr int OFF_NORMS = OFF_COLS + kGroups * 2 * 2 * BN * 4;
+    static constexpr int SMEM = OFF_NORMS + (HEADS ? 2 * HD * 4 : 0) + 1024;
     static constexpr int TMEM_COLS = 2 * BN;
 };
 
@@ -98,30 +106,31 @@ __device__ __forceinline__ void arrive_leader(uint64_t *bar) {
                  : "memory");
 }
 
-// Output of one warpgroup: 64-byte row segments (32 16-bit or 16 f32 columns)
-// staged in shared memory with the 64-byte swizzle, then one TMA store (or
-// f32 reduce-add) per chunk; where the output's base or row stride is not a
-// multiple of 16 bytes, the chunk's elements are written by the warps, a row
-// segment per (half) warp.  Rows past M and columns past N are left alone.
+// Output of one warp (32 rows): 64-byte row segments (32 16-bit or 16 f32
+// columns) staged in shared memory with the 64-byte swizzle, then one TMA store
+// (or f32 reduce-add) per chunk, so a warp waits for no other; where the
+// output's base or row stride is not a multiple of 16 bytes, the warp writes
+// the chunk's elements itself, a row segment at a time.  Rows past M and
+// columns past N are left alone.
 struct Sink {
     const I8Params &p;
     const CUtensorMap *map;
     uint8_t *stage;  // two chunks
-    int r, y0, g;
-    bool elected, tma;
+    int lane, y0;    // y0: first row
+    bool tma;
     int k = 0;
 
     __device__ __forceinline__ uint8_t *acquire() {
         uint8_t *buf = stage + (k & 1) * CHUNK;
-        if (elected && tma) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-        named_bar(1 + g, 128);
+        if (lane == 0 && tma) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        __syncwarp();
         return buf;
     }
     __device__ __forceinline__ void publish(uint8_t *buf, int col) {
         if (tma) fence_proxy_async_smem();
-        named_bar(1 + g, 128);
+        __syncwarp();
         if (tma) {
-            if (elected) {
+            if (lane == 0) {
                 if (p.accumulate)
                     asm volatile(
                         "cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.bulk_group"
@@ -137,14 +146,12 @@ struct Sink {
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
         } else {
-            const int lane = r & 31, w = r >> 5;
             const bool f32 = p.type == kI8F32;
-            const int width = f32 ? 16 : 32;
-            const int c = lane & (width - 1);
+            const int c = lane & (f32 ? 15 : 31);
             const int byte = f32 ? c * 4 : c * 2;
             if (col + c < p.N) {
-                const int rows = min(BM, p.M - y0);
-                for (int i = f32 ? 2 * w + (lane >> 4) : w; i < rows; i += f32 ? 8 : 4) {
+                const int rows = min(32, p.M - y0);
+                for (int i = f32 ? lane >> 4 : 0; i < rows; i += f32 ? 2 : 1) {
                     const uint8_t *src =
                         buf + i * 64 + (((byte >> 4) ^ ((i >> 1) & 3)) << 4) + (byte & 15);
                     const size_t off = (size_t)(y0 + i) * p.ldy + col + c;
@@ -169,7 +176,7 @@ struct Sink {
                 uint8_t *buf = acquire();
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    *reinterpret_cast<float4 *>(buf + r * 64 + ((c ^ ((r >> 1) & 3)) * 16)) =
+                    *reinterpret_cast<float4 *>(buf + lane * 64 + ((c ^ ((lane >> 1) & 3)) * 16)) =
                         make_float4(v[16 * h + 4 * c], v[16 * h + 4 * c + 1],
                                     v[16 * h + 4 * c + 2], v[16 * h + 4 * c + 3]);
                 publish(buf, col + 16 * h);
@@ -180,7 +187,7 @@ struct Sink {
         const bool f16 = p.type == kI8F16;
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<uint4 *>(buf + r * 64 + ((c ^ ((r >> 1) & 3)) * 16)) =
+            *reinterpret_cast<uint4 *>(buf + lane * 64 + ((c ^ ((lane >> 1) & 3)) * 16)) =
                 make_uint4(pack16x2(v[8 * c], v[8 * c + 1], f16),
                            pack16x2(v[8 * c + 2], v[8 * c + 3], f16),
                            pack16x2(v[8 * c + 4], v[8 * c + 5], f16),
@@ -188,52 +195,122 @@ struct Sink {
         publish(buf, col);
     }
     __device__ __forceinline__ void finish() {
-        if (elected && tma) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        if (lane == 0 && tma) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
 };
 
-// 32 accumulators scaled: v = acc * s * t + b.
+// 32 accumulators scaled: v = acc * s * t + b (b null: no bias).
 __device__ __forceinline__ void scale32(float (&v)[32], float s, const float *t, const float *b) {
+    const float2 s2 = make_float2(s, s);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float4 tv = reinterpret_cast<const float4 *>(t)[i];
-        const float4 bv = reinterpret_cast<const float4 *>(b)[i];
-        const float tt[4] = {tv.x, tv.y, tv.z, tv.w}, bb[4] = {bv.x, bv.y, bv.z, bv.w};
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            v[4 * i + u] = fmaf((float)__float_as_int(v[4 * i + u]) * s, tt[u], bb[u]);
+        float4 bv = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (b) bv = reinterpret_cast<const float4 *>(b)[i];
+        const float2 a0 = mul_f32x2(make_float2((float)__float_as_int(v[4 * i]),
+                                                (float)__float_as_int(v[4 * i + 1])),
+                                    s2);
+        const float2 a1 = mul_f32x2(make_float2((float)__float_as_int(v[4 * i + 2]),
+                                                (float)__float_as_int(v[4 * i + 3])),
+                                    s2);
+        const float2 r0 = fma_f32x2(a0, make_float2(tv.x, tv.y), make_float2(bv.x, bv.y));
+        const float2 r1 = fma_f32x2(a1, make_float2(tv.z, tv.w), make_float2(bv.z, bv.w));
+        v[4 * i] = r0.x;
+        v[4 * i + 1] = r0.y;
+        v[4 * i + 2] = r1.x;
+        v[4 * i + 3] = r1.y;
     }
 }
 
 __device__ __forceinline__ void act32(float (&v)[32], int act, bool f32) {
     if (act == kI8None) return;
-    if (act == kI8Silu && !f32) {
+    if (f32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = i8::act_full(v[i], act);
+    } else if (act == kI8Silu) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = epi::silu_fast(v[i]);
+    } else if (act == kI8GeluErf) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = i8::gelu_erf_16(v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = epi::gelu_tanh_fast(v[i]);
+    }
+}
+
+// Whole row segments from registers: N values at y + off (16-bit: packed).
+// 32-byte stores where the address allows, else 16-byte ones, else elements.
+template <int N>
+__device__ __forceinline__ void store_row(const I8Params &p, size_t off, const float (&v)[N]) {
+    if (p.type == kI8F32) {
+        float *o = static_cast<float *>(p.y) + off;
+        if ((reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+#pragma unroll
+            for (int i = 0; i < N / 4; ++i)
+                reinterpret_cast<float4 *>(o)[i] =
+                    make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) o[i] = v[i];
+        }
         return;
     }
+    const bool f16 = p.type == kI8F16;
+    uint16_t *o = static_cast<uint16_t *>(p.y) + off;
+    uint32_t w[N / 2];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = i8::act_full(v[i], act);
+    for (int i = 0; i < N / 2; ++i) w[i] = pack16x2(v[2 * i], v[2 * i + 1], f16);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(o);
+    if ((at & 31) == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 16; ++i)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o + 16 * i),
+                         "r"(w[8 * i]), "r"(w[8 * i + 1]), "r"(w[8 * i + 2]), "r"(w[8 * i + 3]),
+                         "r"(w[8 * i + 4]), "r"(w[8 * i + 5]), "r"(w[8 * i + 6]), "r"(w[8 * i + 7])
+                         : "memory");
+    } else if ((at & 15) == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 8; ++i)
+            reinterpret_cast<uint4 *>(o)[i] =
+                make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            o[2 * i] = (uint16_t)w[i];
+            o[2 * i + 1] = (uint16_t)(w[i] >> 16);
+        }
+    }
 }
 
 // One 128-row x BN accumulator.  cols: this warpgroup's scales [BN] then biases [BN].
-template <int BN, int EPI, int HD>
-__device__ __forceinline__ void epilogue(const I8Params &p, uint32_t tbase, int grow, float s,
-                                         int nb, int g, const float *cols, Sink &sink) {
+template <int BN, int EPI>
+__device__ __forceinline__ void epilogue(const I8Params &p, uint32_t tbase, float s, int nb, int g,
+                                         const float *cols, Sink &sink) {
     const bool f32 = p.type == kI8F32;
+    const float *bias = p.bias ? cols + BN : nullptr;
     if constexpr (EPI == kI8Store) {
+        // Two units of 32 columns per TMEM round trip.
+        constexpr int UNITS = BN / 32 / kGroups;
 #pragma unroll 1
-        for (int c = g; c < BN / 32; c += kGroups) {
-            const int col = nb * BN + c * 32;
-            if (col >= p.N) break;
-            float v[32];
-            tmem_ld32(tbase + c * 32, v);
+        for (int u = 0; u < UNITS; u += 2) {
+            const int c0 = (g * UNITS + u) * 32;
+            if (nb * BN + c0 >= p.N) break;
+            float v[32], w[32];
+            tmem_ld32(tbase + c0, v);
+            if (UNITS > 1) tmem_ld32(tbase + c0 + 32, w);
             tmem_wait_ld();
-            scale32(v, s, cols + c * 32, cols + BN + c * 32);
+            scale32(v, s, cols + c0, bias ? bias + c0 : nullptr);
             act32(v, p.act, f32);
-            sink.put(v, col);
+            sink.put(v, nb * BN + c0);
+            if (UNITS > 1 && nb * BN + c0 + 32 < p.N) {
+                scale32(w, s, cols + c0 + 32, bias ? bias + c0 + 32 : nullptr);
+                act32(w, p.act, f32);
+                sink.put(w, nb * BN + c0 + 32);
+            }
         }
-    } else if constexpr (EPI == kI8Gated) {
+    } else {
+        const float *bias2 = p.bias2 ? cols + BN + BN / 2 : nullptr;
 #pragma unroll 1
         for (int c = g; c < BN / 64; c += kGroups) {
             const int col = nb * (BN / 2) + c * 32;
@@ -242,73 +319,135 @@ __device__ __forceinline__ void epilogue(const I8Params &p, uint32_t tbase, int 
             tmem_ld32(tbase + c * 32, a);
             tmem_ld32(tbase + BN / 2 + c * 32, u);
             tmem_wait_ld();
-            scale32(a, s, cols + c * 32, cols + BN + c * 32);
-            scale32(u, s, cols + BN / 2 + c * 32, cols + BN + BN / 2 + c * 32);
+            scale32(a, s, cols + c * 32, bias ? bias + c * 32 : nullptr);
+            scale32(u, s, cols + BN / 2 + c * 32, bias2 ? bias2 + c * 32 : nullptr);
             act32(a, p.act, f32);
 #pragma unroll
             for (int i = 0; i < 32; ++i) a[i] *= u[i];
             sink.put(a, col);
         }
-    } else {
-        constexpr int HALF = HD / 2;
+    }
+}
+
+// The head form: a warpgroup takes every second head of the tile.  A thread
+// holds its row's whole head in registers, so TMEM is read once.  rope: the
+// row's cos and sin [HD / 2] each (shared memory); norms: q_norm, k_norm [HD].
+template <int BN, int HD>
+__device__ __forceinline__ void epilogue_heads(const I8Params &p, uint32_t tbase, int grow, float s,
+                                               bool bad, int nb, int g, const float *cols,
+                                               const float *rope, const float *norms) {
+    constexpr int HALF = HD / 2, H32 = HALF / 32;
+    const float *bias = p.bias ? cols + BN : nullptr;
 #pragma unroll 1
-        for (int h0 = g * HD; h0 < BN; h0 += kGroups * HD) {
-            const int col0 = nb * BN + h0;
-            if (col0 >= p.N) break;
-            const int head = col0 / HD;
-            const bool is_q = head < p.n_q_heads;
-            const bool rot = head < p.n_q_heads + p.n_kv_heads;
-            float v[HD / 32][32];
+    for (int h0 = g * HD; h0 < BN; h0 += kGroups * HD) {
+        const int col0 = nb * BN + h0;
+        if (col0 >= p.N) break;
+        const int head = col0 / HD;
+        const bool is_q = head < p.n_q_heads;
+        const bool rot = head < p.n_q_heads + p.n_kv_heads;
+        const size_t off = (size_t)grow * p.ldy + col0;
+        float v[HD / 32][32];
 #pragma unroll
-            for (int c = 0; c < HD / 32; ++c) tmem_ld32(tbase + h0 + c * 32, v[c]);
-            tmem_wait_ld();
+        for (int c = 0; c < HD / 32; ++c) tmem_ld32(tbase + h0 + c * 32, v[c]);
+        tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < HD / 32; ++c)
-                scale32(v[c], s, cols + h0 + c * 32, cols + BN + h0 + c * 32);
-            if (rot) {
-                const float *nw = is_q ? p.q_norm : p.k_norm;
-                const int ps = grow < p.M ? __ldg(p.pos + grow) : 0;
-                const bool bad = ps < 0 || ps >= p.n_pos;
-                if (bad) set_error(p.err, kErrBadPosition);
-                float inv = bad ? i8::nan_f() : 1.0f;
-                if (nw) {
-                    float ss = 0.0f;
+        for (int c = 0; c < HD / 32; ++c)
+            scale32(v[c], s, cols + h0 + c * 32, bias ? bias + h0 + c * 32 : nullptr);
+        if (rot) {
+            const bool normed = is_q ? p.q_norm != nullptr : p.k_norm != nullptr;
+            float inv = bad ? i8::nan_f() : 1.0f;
+            if (normed) {
+                float2 q[4] = {};
 #pragma unroll
-                    for (int c = 0; c < HD / 32; ++c)
+                for (int c = 0; c < HD / 32; ++c)
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) ss = fmaf(v[c][i], v[c][i], ss);
-                    inv *= 1.0f / sqrtf(ss / (float)HD + p.eps);
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 x = make_float2(v[c][2 * i], v[c][2 * i + 1]);
+                        q[i & 3] = fma_f32x2(x, x, q[i & 3]);
+                    }
+                const float2 t = add_f32x2(add_f32x2(q[0], q[1]), add_f32x2(q[2], q[3]));
+                inv *= 1.0f / sqrtf((t.x + t.y) / (float)HD + p.eps);
+            }
+            const float *nw = norms + (is_q ? 0 : HD);
+            const float2 inv2 = make_float2(inv, inv);
+#pragma unroll
+            for (int i = 0; i < HALF / 4; ++i) {
+                const float4 cv = reinterpret_cast<const float4 *>(rope)[i];
+                const float4 sv = reinterpret_cast<const float4 *>(rope + HALF)[i];
+                float4 w1 = make_float4(1.0f, 1.0f, 1.0f, 1.0f), w2 = w1;
+                if (normed) {
+                    w1 = reinterpret_cast<const float4 *>(nw)[i];
+                    w2 = reinterpret_cast<const float4 *>(nw + HALF)[i];
                 }
-                const float4 *cs =
-                    reinterpret_cast<const float4 *>(p.cos + (size_t)(bad ? 0 : ps) * HALF);
-                const float4 *sn =
-                    reinterpret_cast<const float4 *>(p.sin + (size_t)(bad ? 0 : ps) * HALF);
 #pragma unroll
-                for (int i = 0; i < HALF / 4; ++i) {
-                    const float4 cv = __ldg(cs + i), sv = __ldg(sn + i);
-                    float4 w1 = make_float4(1.0f, 1.0f, 1.0f, 1.0f), w2 = w1;
-                    if (nw) {
-                        w1 = __ldg(reinterpret_cast<const float4 *>(nw) + i);
-                        w2 = __ldg(reinterpret_cast<const float4 *>(nw + HALF) + i);
+                for (int u = 0; u < 2; ++u) {
+                    const int e = 4 * i + 2 * u;
+                    float(&A)[32] = v[e / 32], (&B)[32] = v[H32 + e / 32];
+                    const int j = e % 32;
+                    const float2 c2 = u ? make_float2(cv.z, cv.w) : make_float2(cv.x, cv.y);
+                    const float2 s2 = u ? make_float2(sv.z, sv.w) : make_float2(sv.x, sv.y);
+                    float2 a = mul_f32x2(make_float2(A[j], A[j + 1]), inv2);
+                    float2 b = mul_f32x2(make_float2(B[j], B[j + 1]), inv2);
+                    if (normed) {
+                        a = mul_f32x2(a, u ? make_float2(w1.z, w1.w) : make_float2(w1.x, w1.y));
+                        b = mul_f32x2(b, u ? make_float2(w2.z, w2.w) : make_float2(w2.x, w2.y));
                     }
-                    const float cc[4] = {cv.x, cv.y, cv.z, cv.w}, sc[4] = {sv.x, sv.y, sv.z, sv.w};
-                    const float wa[4] = {w1.x, w1.y, w1.z, w1.w}, wb[4] = {w2.x, w2.y, w2.z, w2.w};
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        constexpr int H32 = HALF / 32;
-                        const int e = 4 * i + u;
-                        float &a = v[e / 32][e % 32], &b = v[H32 + e / 32][e % 32];
-                        const float x1 = a * inv * wa[u], x2 = b * inv * wb[u];
-                        a = x1 * cc[u] - x2 * sc[u];
-                        b = x2 * cc[u] + x1 * sc[u];
-                    }
+                    const float2 ns = make_float2(-s2.x, -s2.y);
+                    const float2 r1 = fma_f32x2(b, ns, mul_f32x2(a, c2));
+                    const float2 r2 = fma_f32x2(a, s2, mul_f32x2(b, c2));
+                    A[j] = r1.x;
+                    A[j + 1] = r1.y;
+                    B[j] = r2.x;
+                    B[j + 1] = r2.y;
                 }
             }
+        }
+        if (grow < p.M) {
 #pragma unroll
-            for (int c = 0; c < HD / 32; ++c) sink.put(v[c], col0 + c * 32);
+            for (int c = 0; c < HD / 32; ++c) store_row<32>(p, off + c * 32, v[c]);
         }
     }
 }
+
+// Tiles of one SM pair, in order.  Head form: a run of neighbouring tiles, row
+// blocks outermost, so that the rotary rows change seldom.  Otherwise the pairs
+// take turns over groups of kRaster row blocks, columns outermost within a
+// group: the pairs' tiles of one moment then share both operands (with row
+// blocks outermost they would share one row block and read 74 different weight
+// tiles, all of a large matrix per row block).
+constexpr int kRaster = 8;
+
+template <int EPI>
+struct Tiles {
+    int m_blocks, n_blocks, next, end, step;
+    __device__ Tiles(int mb, int nb, int pair, int n_pairs) : m_blocks(mb), n_blocks(nb) {
+        const int total = mb * nb;
+        if (EPI == kI8Heads) {
+            next = (int)((long long)total * pair / n_pairs);
+            end = (int)((long long)total * (pair + 1) / n_pairs);
+            step = 1;
+        } else {
+            next = pair;
+            end = total;
+            step = n_pairs;
+        }
+    }
+    __device__ __forceinline__ bool pop(int &mb, int &nb) {
+        if (next >= end) return false;
+        if (EPI == kI8Heads) {
+            mb = next / n_blocks;
+            nb = next % n_blocks;
+        } else {
+            const int group = next / (kRaster * n_blocks);
+            const int rows = min(kRaster, m_blocks - group * kRaster);
+            const int r = next - group * kRaster * n_blocks;
+            mb = group * kRaster + r % rows;
+            nb = r / rows;
+        }
+        next += step;
+        return true;
+    }
+};
 
 template <int BN, int EPI, int HD>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
@@ -316,7 +455,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                    const __grid_constant__ CUtensorMap tmB2,
                    const __grid_constant__ CUtensorMap tmOut, const I8Params p, const int tma_out) {
     extern __shared__ uint8_t smem_raw[];
-    using CF = Cfg<BN>;
+    using CF = Cfg<BN, EPI, HD>;
     constexpr int STAGES = CF::STAGES;
     __shared__ __align__(8) uint64_t full_bar[STAGES];
     __shared__ __align__(8) uint64_t empty_bar[STAGES];
@@ -336,10 +475,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     constexpr int TN = EPI == kI8Gated ? BN / 2 : BN;  // output columns per tile
     const int m_blocks = (p.M + 2 * BM - 1) / (2 * BM);
     const int n_blocks = (p.N + TN - 1) / TN;
-    const int num_tiles = m_blocks * n_blocks;
     const int k_blocks = (p.K + BK - 1) / BK;
     const int pair = blockIdx.x >> 1;
     const int n_pairs = gridDim.x >> 1;
+
+    Tiles<EPI> tiles(m_blocks, n_blocks, pair, n_pairs);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
@@ -381,8 +521,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const CUtensorMap *mb_map = EPI == kI8Gated && !leader ? &tmB2 : &tmB;
             int it = 0;
             bool ok = true;
-            for (int tile = pair; ok && tile < num_tiles; tile += n_pairs) {
-                const int mb = tile / n_blocks, nb = tile % n_blocks;
+            int mb, nb;
+            while (ok && tiles.pop(mb, nb)) {
                 const int brow = EPI == kI8Gated ? nb * TN : nb * BN + (int)rank * (BN / 2);
                 for (int kb = 0; kb < k_blocks; ++kb) {
                     const int s = it % STAGES;
@@ -411,7 +551,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             constexpr uint32_t IDESC = idesc_i8(2 * BM, BN);
             int it = 0, lt = 0;
             bool ok = true;
-            for (int tile = pair; ok && tile < num_tiles; tile += n_pairs, ++lt) {
+            int mb, nb;
+            for (; ok && tiles.pop(mb, nb); ++lt) {
                 const int a = lt & 1;
                 const uint32_t aph = (lt >> 1) & 1;
                 if (!mbar_wait(&tempty_bar[a], aph ^ 1, p.err, &abort_sh)) {
@@ -456,20 +597,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int g = (warp - 2) >> 2;
         const int row = q * 32 + lane;
         const int gt = (warp - 2 - 4 * g) * 32 + lane;  // thread of the warpgroup
-        float *cols = reinterpret_cast<float *>(smem + CF::OFF_COLS) + g * 2 * BN;
-        Sink sink{p, &tmOut, smem + CF::OFF_STAGING + g * 2 * CHUNK, row, 0, g, gt == 0,
-                  tma_out != 0};
-        int lt = 0;
-        for (int tile = pair; tile < num_tiles; tile += n_pairs, ++lt) {
+        const int et = (warp - 2) * 32 + lane;          // thread of the epilogue
+        float *cols0 = reinterpret_cast<float *>(smem + CF::OFF_COLS) + g * 4 * BN;
+        Sink sink{p, &tmOut, smem + CF::OFF_STAGING + (warp - 2) * 2 * CHUNK, lane, 0, tma_out != 0};
+        float *rope = reinterpret_cast<float *>(smem + CF::OFF_STAGING);
+        float *norms = reinterpret_cast<float *>(smem + CF::OFF_NORMS);
+        if (EPI == kI8Heads) {
+            for (int i = et; i < HD; i += 128 * kGroups) {
+                norms[i] = p.q_norm ? __ldg(p.q_norm + i) : 1.0f;
+                norms[HD + i] = p.k_norm ? __ldg(p.k_norm + i) : 1.0f;
+            }
+        }
+        int lt = 0, mb, nb, rope_mb = -1;
+        bool bad = false;
+        for (; tiles.pop(mb, nb); ++lt) {
             const int a = lt & 1;
             const uint32_t aph = (lt >> 1) & 1;
-            const int mb = tile / n_blocks, nb = tile % n_blocks;
             const int y0 = mb * 2 * BM + (int)rank * BM;
             const int grow = y0 + row;
-            // The tile's scales and biases, fetched while its products run.  The
-            // barrier ahead of the writes is past every read of the last tile's.
+            // Fetched while the tile's products run: the row's scale, the
+            // columns' scales and biases (in turns of two buffers: a thread
+            // passes the barrier below only after the tile before last).
             const float s = grow < p.M ? __ldg(p.xs + grow) : 0.0f;
-            named_bar(1 + g, 128);
+            float *cols = cols0 + a * 2 * BN;
             for (int c = gt; c < BN; c += 128) {
                 const bool second = EPI == kI8Gated && c >= TN;
                 const int col = nb * TN + (second ? c - TN : c);
@@ -477,17 +627,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 cols[c] = col < p.N ? __ldg(t + col) : 0.0f;
                 cols[BN + c] = b && col < p.N ? __ldg(b + col) : 0.0f;
             }
-            // One verdict for the warpgroup: its barriers below need all of it.
-            if (!named_bar_and(1 + g, 128, mbar_wait(&tfull_bar[a], aph, p.err, &abort_sh))) break;
+            if constexpr (EPI == kI8Heads) {
+                if (mb != rope_mb) {
+                    // The rotary rows of this row block: a warp copies 16 rows,
+                    // one at a time.  All warps are past their last reads.
+                    rope_mb = mb;
+                    named_bar(1 + kGroups, 128 * kGroups);
+                    const int ps = grow < p.M ? __ldg(p.pos + grow) : 0;
+                    bad = ps < 0 || ps >= p.n_pos;
+                    if (bad) set_error(p.err, kErrBadPosition);
+                    constexpr int V = HD / 4;  // float4 per row, cos then sin
+                    for (int i = 0; i < 16; ++i) {
+                        const int r = q * 32 + g * 16 + i;
+                        int rp = __shfl_sync(0xffffffffu, ps, g * 16 + i);
+                        if (rp < 0 || rp >= p.n_pos) rp = 0;
+                        if (lane < V) {
+                            const float *src = (lane < V / 2 ? p.cos : p.sin) + (size_t)rp * (HD / 2);
+                            reinterpret_cast<float4 *>(rope + r * CF::ROPE_LD)[lane] =
+                                __ldg(reinterpret_cast<const float4 *>(src) + lane % (V / 2));
+                        }
+                    }
+                    named_bar(1 + kGroups, 128 * kGroups);
+                }
+            }
+            // One verdict for the warpgroup (its barriers need all of it), and
+            // in the head form for both.
+            const bool ok = mbar_wait(&tfull_bar[a], aph, p.err, &abort_sh);
+            if (!(EPI == kI8Heads ? named_bar_and(1 + kGroups, 128 * kGroups, ok)
+                                  : named_bar_and(1 + g, 128, ok)))
+                break;
             tc_fence_after();
             const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + a * BN;
-            sink.y0 = y0;
-            if (y0 < p.M) epilogue<BN, EPI, HD>(p, tbase, grow, s, nb, g, cols, sink);
+            sink.y0 = y0 + q * 32;
+            if constexpr (EPI == kI8Heads) {
+                if (y0 < p.M)
+                    epilogue_heads<BN, HD>(p, tbase, grow, s, bad, nb, g, cols,
+                                           rope + row * CF::ROPE_LD, norms);
+            } else {
+                if (sink.y0 < p.M) epilogue<BN, EPI>(p, tbase, s, nb, g, cols, sink);
+            }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) arrive_leader(&tempty_bar[a]);
         }
-        sink.finish();
+        if (EPI != kI8Heads) sink.finish();
     }
 
     tc_fence_before();
@@ -513,19 +696,20 @@ int launch(const I8Params &p, int num_sms, cudaStream_t stream) {
     if (EPI == kI8Gated && make_map_ld(&mb2, p.w2, p.N, p.K, p.ldw2, BN / 2, BK, SW, U8, 1))
         return -1;
     const int esz = p.type == kI8F32 ? 4 : 2;
-    const bool tma = (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && (p.ldy * esz) % 16 == 0;
+    const bool tma = EPI != kI8Heads && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 &&
+                     (p.ldy * esz) % 16 == 0;
     mo = ma;
-    if (tma && make_map_ld(&mo, p.y, p.M, p.N, p.ldy, 128, 64 / esz, CU_TENSOR_MAP_SWIZZLE_64B,
+    if (tma && make_map_ld(&mo, p.y, p.M, p.N, p.ldy, 32, 64 / esz, CU_TENSOR_MAP_SWIZZLE_64B,
                            p.type == kI8F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                            : p.type == kI8BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                            esz))
         return -1;
-    CK((set_smem_once<i8_gemm_kernel<BN, EPI, HD>>(Cfg<BN>::SMEM)));
+    CK((set_smem_once<i8_gemm_kernel<BN, EPI, HD>>(Cfg<BN, EPI, HD>::SMEM)));
     constexpr int TN = EPI == kI8Gated ? BN / 2 : BN;
     const long long tiles = (long long)((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + TN - 1) / TN);
     const int grid = (int)std::min<long long>(2 * tiles, num_sms & ~1);
-    LAUNCH(launch_k(i8_gemm_kernel<BN, EPI, HD>, dim3(grid), dim3(kThreads), Cfg<BN>::SMEM, stream,
+    LAUNCH(launch_k(i8_gemm_kernel<BN, EPI, HD>, dim3(grid), dim3(kThreads), (Cfg<BN, EPI, HD>::SMEM), stream,
                     ma, mb, mb2, mo, p, tma ? 1 : 0));
     return 0;
 }

@@ -3,7 +3,8 @@
 // up to 16384 columns; longer ones are read twice) and written once at a byte
 // per value.
 //
-// Rounding.  The code of a value is the nearest integer of v / s.  In f32 the
+// Rounding.  The code of a value is the nearest integer of v / s (s = amax / 127,
+// both quotients in f64; ties to even).  In f32 the
 // quotient is off by a few units in the last place (the product x * norm, the
 // reciprocal and the product with it: 4 x 2^-24 x 127 < 4e-5), which matters
 // only next to the border of two codes; there, about one value in 10^4, it is
@@ -65,44 +66,78 @@ __device__ __forceinline__ void load8_norm(const float *w, int c, int K, bool ve
 // The residue of the f32 product x * w = p (exact unless it underflows).
 __device__ __forceinline__ float residue(float x, float w, float p) { return fmaf(x, w, -p); }
 
-// Codes of eight values (p, plus the residues of p = x * g with a norm) of a
-// row whose largest magnitude is amax + amax_lo; written as 8 bytes, or as
-// fewer at the row's end.
+// max(m, |v|), NaN if either is.
+__device__ __forceinline__ float max_abs(float m, float v) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(v)));
+    return r;
+}
+
+// 1.5 x 2^23: adding it leaves the nearest integer in the low bits of the sum
+// (ties to even), two's complement in the lowest byte.
+constexpr float kRound = 12582912.0f;
+
+__device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d) {
+    const uint32_t lo = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
+}
+
+// Codes of eight values (p = x, or x * g with a norm) of a row whose largest
+// magnitude is amax + amax_lo; written as 8 bytes, or as fewer at the row's end.
 template <bool NORM>
 __device__ __forceinline__ void put8(const float (&x)[8], const float (&g)[8], float inv,
                                      float amax, float amax_lo, int8_t *q, int c, int K) {
-    int code[8];
-    bool near = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float p = NORM ? x[i] * g[i] : x[i];
-        const float t = p * inv;
-        const float f = rintf(t);
-        near |= fabsf(fabsf(t - f) - 0.5f) < kTieBand;
-        code[i] = (int)f;
-    }
-    if (near || inv == 0.0f) {
-        // In f64; also the rows so small that 127 / amax is not a finite f32
-        // (inv = 0 marks them).
-        const double s = ((double)amax + (double)amax_lo) / 127.0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const double v = NORM ? (double)x[i] * (double)g[i] : (double)x[i];
-            code[i] = (int)rint(v / s);
-        }
-    }
-    uint32_t w0 = 0, w1 = 0;
+    float code[8];
+    float far = 0.0f;  // largest distance from a code
+    const float2 inv2 = make_float2(inv, inv), up = make_float2(kRound, kRound),
+                 down = make_float2(-kRound, -kRound);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        w0 |= (uint32_t)(code[i] & 0xFF) << (8 * i);
-        w1 |= (uint32_t)(code[4 + i] & 0xFF) << (8 * i);
+        float2 t = make_float2(x[2 * i], x[2 * i + 1]);
+        if (NORM) t = mul_f32x2(t, make_float2(g[2 * i], g[2 * i + 1]));
+        t = mul_f32x2(t, inv2);
+        const float2 f = add_f32x2(t, up);
+        const float2 d = add_f32x2(t, mul_f32x2(add_f32x2(f, down), make_float2(-1.0f, -1.0f)));
+        far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
+        code[2 * i] = f.x;
+        code[2 * i + 1] = f.y;
+    }
+    uint32_t w0 = low_bytes(code[0], code[1], code[2], code[3]);
+    uint32_t w1 = low_bytes(code[4], code[5], code[6], code[7]);
+    if (far > 0.5f - kTieBand) {
+        // In f64, one value after another (a rare path, kept small).
+        const double s = ((double)amax + (double)amax_lo) / 127.0;
+        uint32_t near = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float d = (NORM ? x[i] * g[i] : x[i]) * inv - (code[i] - kRound);
+            near |= (fabsf(d) > 0.5f - 2.0f * kTieBand ? 1u : 0u) << i;
+        }
+#pragma unroll 1
+        for (; near; near &= near - 1) {
+            const int j = __ffs(near) - 1;
+            float xj = x[0], gj = g[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i)
+                if (i == j) {
+                    xj = x[i];
+                    if (NORM) gj = g[i];
+                }
+            const double v = NORM ? (double)xj * (double)gj : (double)xj;
+            const uint32_t byte = (uint32_t)(int)rint(v / s) & 0xFF;
+            const int sh = 8 * (j & 3);
+            const uint32_t w = ((j < 4 ? w0 : w1) & ~(0xFFu << sh)) | byte << sh;
+            if (j < 4) w0 = w;
+            else w1 = w;
+        }
     }
     if (c + 8 <= K) {
         *reinterpret_cast<uint2 *>(q + c) = make_uint2(w0, w1);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (c + i < K) q[c + i] = (int8_t)code[i];
+            if (c + i < K) q[c + i] = (int8_t)((i < 4 ? w0 : w1) >> (8 * (i & 3)));
     }
 }
 
@@ -126,14 +161,13 @@ __global__ void __launch_bounds__((W > 8 ? W : 8) * 32)
     const int t = wr * 32 + lane;
     constexpr int NR = NV > 0 ? NV : 1;
     float v[NR][8], g[NR][8];
-    uint32_t mx = 0;
+    float mv = 0.0f;
     float ss = 0.0f;
     auto stats = [&](const float(&a)[8], const float(&b)[8]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             if (NORM) ss = fmaf(a[i], a[i], ss);
-            // Magnitudes compare as unsigned integers, NaN above infinity.
-            mx = max(mx, __float_as_uint(NORM ? a[i] * b[i] : a[i]) & 0x7FFFFFFFu);
+            mv = max_abs(mv, NORM ? a[i] * b[i] : a[i]);
         }
     };
     if (live) {
@@ -154,7 +188,9 @@ __global__ void __launch_bounds__((W > 8 ? W : 8) * 32)
             }
         }
     }
-    mx = __reduce_max_sync(0xffffffffu, mx);
+    // Magnitudes compare as unsigned integers, NaN above infinity.
+    const uint32_t mine = __float_as_uint(mv);
+    uint32_t mx = __reduce_max_sync(0xffffffffu, mine);
     if (NORM) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
@@ -190,7 +226,7 @@ __global__ void __launch_bounds__((W > 8 ? W : 8) * 32)
                 }
             }
         };
-        if (live) {
+        if (live && mine == mx) {
             if (NV > 0) {
 #pragma unroll
                 for (int k = 0; k < NR; ++k) resid(v[k], g[k]);
@@ -232,7 +268,17 @@ __global__ void __launch_bounds__((W > 8 ? W : 8) * 32)
         if (NORM) sc /= sqrt((double)ss / (double)K + (double)eps);
         s[row] = (float)sc;
     }
-    const float inv = amax > 1e-30f ? 127.0f / amax : 0.0f;
+    if (amax < 1e-30f) {
+        // 127 / amax may pass f32: such rows go through f64, a value at a time.
+        const double sc = ((double)amax + (double)amax_lo) / 127.0;
+        for (int c = t; c < K; c += W * 32) {
+            double v = (double)load1<TYPE>(x, off + c);
+            if (NORM) v *= (double)norm[c];
+            qr[c] = (int8_t)(int)rint(v / sc);
+        }
+        return;
+    }
+    const float inv = 127.0f / amax;
     if (NV > 0) {
 #pragma unroll
         for (int k = 0; k < NR; ++k) {
