@@ -1,44 +1,84 @@
 // Epilogue arithmetic shared by the 8-bit integer kernels.
 //
-// Activations of f32 results are computed with the full-precision functions;
-// 16-bit results take forms of two MUFU operations whose error (a few 2^-24 of
-// the argument) is far below their rounding: the epilogue shares the SM with a
-// tile's products (4096 cycles at K = 1024), which erff for its 32768 values
-// alone would pass (8192 x 4096 x 1024 rows with GELU: 88 us with erff).
+// Activations work on pairs of values in packed f32 arithmetic with two
+// special-function operations each (a power of two and a reciprocal), for every
+// output type: the epilogue shares the SM with the next tile's products (4096
+// cycles at K = 1024 for 32768 values), and the library's erff, tanhf and expf
+// in one kernel outgrow the instruction cache as well (8192 x 4096 x 1024 with
+// GELU: 64 us).
 #pragma once
 
-#include "gemm_epi.cuh"
 #include "int8.cuh"
 #include "ptx.cuh"
 
 namespace fb {
 namespace i8 {
 
-__device__ __forceinline__ float act_full(float x, int act) {
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float2 both(float c) { return make_float2(c, c); }
+
+// GELU of two values by the normal distribution's upper tail, h = (1 - erf(z)) / 2
+// at z = |x| / sqrt 2, as max(x, 0) - |x| h.  1 - erf(z) = P(t) e^(-z^2) with t =
+// 1 / (1 + 0.4 z) and P of degree 6 without a constant, fitted here (weighted
+// least squares in t, z <= 7): x h is off by at most 2e-8 plus rounding.
+__device__ __forceinline__ float2 gelu_erf(float2 x) {
+    // (finite, so that an infinite x gives itself or 0)
+    const float2 ax = make_float2(fminf(fabsf(x.x), 3.4e38f), fminf(fabsf(x.y), 3.4e38f));
+    const float2 den = fma_f32x2(ax, both(0.28284271f), both(1.0f));
+    const float2 t = make_float2(rcp_approx(den.x), rcp_approx(den.y));
+    float2 a = fma_f32x2(t, both(0.5f * -0.20369884f), both(0.5f * 0.7232648f));
+    a = fma_f32x2(a, t, both(0.5f * -0.3939358f));
+    a = fma_f32x2(a, t, both(0.5f * 0.48692873f));
+    a = fma_f32x2(a, t, both(0.5f * 0.15432052f));
+    a = fma_f32x2(a, t, both(0.5f * 0.23312044f));
+    // e^(-x^2 / 2) as a power of two.
+    const float2 e = mul_f32x2(mul_f32x2(x, both(-0.72134752f)), x);
+    const float2 h = mul_f32x2(mul_f32x2(a, t), make_float2(ex2_approx(e.x), ex2_approx(e.y)));
+    return fma_f32x2(make_float2(-ax.x, -ax.y), h, make_float2(fmaxf(x.x, 0.0f), fmaxf(x.y, 0.0f)));
+}
+
+// x / (1 + d) of two values.
+__device__ __forceinline__ float2 over_1p(float2 x, float2 d) {
+    d = add_f32x2(d, both(1.0f));
+    return mul_f32x2(x, make_float2(rcp_approx(d.x), rcp_approx(d.y)));
+}
+
+// SiLU, x / (1 + 2^e), e = -x log2(e): e in two parts (its rounding alone would
+// be off by |x| 2^-24 of the result for negative x).
+__device__ __forceinline__ float2 silu(float2 x) {
+    const float2 e = mul_f32x2(x, both(-1.44269504f));
+    const float2 ne = make_float2(-e.x, -e.y);
+    const float2 lo = fma_f32x2(x, both(-1.92596299e-8f), fma_f32x2(x, both(-1.44269504f), ne));
+    const float2 w = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+    // (an infinite power times a zero or infinite lo would be NaN)
+    const float2 cor = mul_f32x2(lo, both(0.69314718f));
+    const float2 wf = make_float2(fminf(w.x, 3.0e38f), fminf(w.y, 3.0e38f));
+    return over_1p(x, fma_f32x2(wf, cor, w));
+}
+
+// GELU, tanh form: 0.5 (1 + tanh(v)) = 1 / (1 + 2^e), v = sqrt(2 / pi) (x +
+// 0.044715 x^3), e = -2 log2(e) v.
+__device__ __forceinline__ float2 gelu_tanh(float2 x) {
+    const float2 k = fma_f32x2(mul_f32x2(x, x), both(-0.1029432f), both(-2.3022082f));
+    const float2 e = mul_f32x2(x, k);
+    return over_1p(x, make_float2(ex2_approx(e.x), ex2_approx(e.y)));
+}
+
+__device__ __forceinline__ float2 act2(float2 x, int act) {
     switch (act) {
-    case kI8Silu: return x / (1.0f + expf(-x));
-    case kI8GeluErf: return epi::gelu_erf(x);
-    case kI8GeluTanh: return epi::gelu_tanh(x);
+    case kI8Silu: return silu(x);
+    case kI8GeluErf: return gelu_erf(x);
+    case kI8GeluTanh: return gelu_tanh(x);
     }
     return x;
 }
 
-// GELU by the normal distribution's upper tail, h = (1 - erf(z)) / 2 at z = |x| /
-// sqrt 2, as x h or x - x h.  1 - erf(z) = t (a1 + t (a2 + ... + t a5)) e^(-z^2),
-// t = 1 / (1 + p z): Abramowitz and Stegun, 7.1.26, off by at most 1.5e-7.
-__device__ __forceinline__ float gelu_erf_16(float x) {
-    const float ax = fabsf(x);
-    const float t = __fdividef(1.0f, fmaf(0.3275911f * 0.70710678f, ax, 1.0f));
-    float a = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
-    a = fmaf(a, t, 0.5f * 1.421413741f);
-    a = fmaf(a, t, 0.5f * -0.284496736f);
-    a = fmaf(a, t, 0.5f * 0.254829592f);
-    // e^(-x^2 / 2) as a power of two.
-    const float h = a * t * ex2_approx(x * x * -0.72134752f);
-    const float xh = ax * h;
-    return x > 0.0f ? x - xh : -xh;
-}
-
+__device__ __forceinline__ float act1(float x, int act) { return act2(make_float2(x, x), act).x; }
 
 __device__ __forceinline__ float nan_f() { return __uint_as_float(0x7FC00000u); }
 

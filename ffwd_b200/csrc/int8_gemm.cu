@@ -8,10 +8,9 @@
 // its 128 output rows in TMEM, in two accumulators, so a tile's epilogue runs
 // under the next tile's products.  In the gated form the leader's half of the
 // weight rows are the gate's and its peer's the up projection's, so matching
-// columns meet in one accumulator.  Roles per CTA (320 threads): warp 0 TMA
-// producer, warp 1 TMEM allocation and (leader) MMA issue, warps 2-9 epilogue
-// in two warpgroups that split the columns.  No TMA load uses multicast.
-#include "gemm_epi.cuh"
+// columns meet in one accumulator.  Roles per CTA : warp 0 TMA
+// producer, warp 1 TMEM allocation and (leader) MMA issue, the other warps the
+// epilogue, in warpgroups that split the columns.  No TMA load uses multicast.
 #include "host_util.h"
 #include "int8.cuh"
 #include "int8_epi.cuh"
@@ -25,8 +24,6 @@ namespace {
 
 constexpr int BM = 128;       // rows per CTA
 constexpr int BK = 128;       // bytes of K per stage
-constexpr int kGroups = 2;    // epilogue warpgroups
-constexpr int kThreads = 64 + 128 * kGroups;
 constexpr int A_BYTES = BM * BK;
 constexpr int CHUNK = 2048;   // 32 rows x 64 bytes of output
 constexpr uint32_t kPeerMask = 0xFEFFFFFFu;  // clears the CTA-rank bit: leader's copy
@@ -34,7 +31,9 @@ constexpr uint32_t kPeerMask = 0xFEFFFFFFu;  // clears the CTA-rank bit: leader'
 // Shared memory.  The head form keeps the rotary rows of the CTA's 128 rows
 // (cos and sin, f32, each row padded by 16 bytes so that 32 lanes reading 16
 // bytes of a row each meet no bank twice) and writes its heads straight from
-// registers; the others stage 2 KB of output per epilogue warp, twice.
+// registers; the others stage 2 KB of output per epilogue warp.  The head form
+// and the gated form have two epilogue warpgroups (a thread holds a whole head,
+// or 32 gate and 32 up sums), the plain one four.
 template <int BN, int EPI, int HD>
 struct Cfg {
     static constexpr bool HEADS = EPI == kI8Heads;
@@ -42,11 +41,15 @@ struct Cfg {
     static constexpr int STAGE = A_BYTES + B_BYTES;
     static constexpr int STAGES = HEADS ? (BN == 256 ? 4 : 5) : BN == 256 ? 5 : BN == 128 ? 7 : 8;
     static constexpr int OFF_STAGING = STAGES * STAGE;
+    static constexpr int GROUPS = EPI == kI8Store ? 4 : 2;  // epilogue warpgroups
+    static constexpr int THREADS = 64 + 128 * GROUPS;
     static constexpr int ROPE_LD = HD + 4;  // floats
-    static constexpr int STAGING = HEADS ? BM * ROPE_LD * 4 : 4 * kGroups * 2 * CHUNK;
-    // Per warpgroup, twice: the tile's scales and biases.
+    static constexpr int STAGING = HEADS ? BM * ROPE_LD * 4 : 4 * GROUPS * CHUNK;
+    // Per warpgroup, twice: the scales and biases of its columns of the tile.
+    static constexpr int MIN_COLS = EPI == kI8Gated ? 64 : 32;  // of one unit
+    static constexpr int GCOLS = HEADS ? 128 : BN / GROUPS < MIN_COLS ? MIN_COLS : BN / GROUPS;
     static constexpr int OFF_COLS = OFF_STAGING + STAGING;
-    static constexpr int OFF_NORMS = OFF_COLS + kGroups * 2 * 2 * BN * 4;
+    static constexpr int OFF_NORMS = OFF_COLS + GROUPS * 2 * 2 * GCOLS * 4;
     static constexpr int SMEM = OFF_NORMS + (HEADS ? 2 * HD * 4 : 0) + 1024;
     static constexpr int TMEM_COLS = 2 * BN;
 };
@@ -99,11 +102,25 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t *bar) {
         : "memory");
 }
 
+// Arrive on the leader CTA's copy of `bar`.  It hands over TMEM that this
+// thread's completed loads have read, no memory: a release at cluster scope
+// would wait for the thread's earlier stores (measured at 1500 cycles a tile).
 __device__ __forceinline__ void arrive_leader(uint64_t *bar) {
     uint32_t remote;
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(remote) : "r"(smem_u32(bar)));
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote)
-                 : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
+}
+
+// Neighbouring values packed in the 16-bit type (one branch for all of them).
+template <int N>
+__device__ __forceinline__ void pack32(uint32_t (&w)[N], const float (&v)[2 * N], bool f16) {
+    if (f16) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = pack_f16x2(v[2 * i], v[2 * i + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+    }
 }
 
 // Output of one warp (32 rows): 64-byte row segments (32 16-bit or 16 f32
@@ -115,16 +132,14 @@ __device__ __forceinline__ void arrive_leader(uint64_t *bar) {
 struct Sink {
     const I8Params &p;
     const CUtensorMap *map;
-    uint8_t *stage;  // two chunks
+    uint8_t *stage;  // one chunk
     int lane, y0;    // y0: first row
     bool tma;
-    int k = 0;
 
     __device__ __forceinline__ uint8_t *acquire() {
-        uint8_t *buf = stage + (k & 1) * CHUNK;
-        if (lane == 0 && tma) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        if (lane == 0 && tma) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncwarp();
-        return buf;
+        return stage;
     }
     __device__ __forceinline__ void publish(uint8_t *buf, int col) {
         if (tma) fence_proxy_async_smem();
@@ -165,7 +180,6 @@ struct Sink {
                 }
             }
         }
-        ++k;
     }
     // 32 columns [col, col + 32) of this thread's row.
     __device__ __forceinline__ void put(const float (&v)[32], int col) {
@@ -183,15 +197,13 @@ struct Sink {
             }
             return;
         }
+        uint32_t w[16];
+        pack32(w, v, p.type == kI8F16);
         uint8_t *buf = acquire();
-        const bool f16 = p.type == kI8F16;
 #pragma unroll
         for (int c = 0; c < 4; ++c)
             *reinterpret_cast<uint4 *>(buf + lane * 64 + ((c ^ ((lane >> 1) & 3)) * 16)) =
-                make_uint4(pack16x2(v[8 * c], v[8 * c + 1], f16),
-                           pack16x2(v[8 * c + 2], v[8 * c + 3], f16),
-                           pack16x2(v[8 * c + 4], v[8 * c + 5], f16),
-                           pack16x2(v[8 * c + 6], v[8 * c + 7], f16));
+                make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
         publish(buf, col);
     }
     __device__ __forceinline__ void finish() {
@@ -199,7 +211,45 @@ struct Sink {
     }
 };
 
-// 32 accumulators scaled: v = acc * s * t + b (b null: no bias).
+// 32 integer sums (as bits) to f32.  The conversion instruction runs at a
+// sixteenth of the arithmetic's rate, so sums below 2^22 in magnitude, all but contrived ones, go
+// through the f32 1.5 x 2^23 + sum, whose bits are those of 1.5 x 2^23 plus
+// the sum; the values whose bits leave its binade are converted.
+template <int R>
+__device__ __forceinline__ void to_f32(float (&v)[R][32]) {
+    constexpr int kBias = 0x4B400000;  // 1.5 x 2^23
+    int out = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const int b = __float_as_int(v[r][i]) + kBias;
+            out |= b ^ 0x4B000000;
+            v[r][i] = __int_as_float(b);
+        }
+    if ((uint32_t)out < 0x800000u) {
+        const float2 down = make_float2(-12582912.0f, -12582912.0f);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float2 f = add_f32x2(make_float2(v[r][2 * i], v[r][2 * i + 1]), down);
+                v[r][2 * i] = f.x;
+                v[r][2 * i + 1] = f.y;
+            }
+    } else {
+        // volatile: a branch, not both sides and a choice (in twice the registers)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                asm volatile("cvt.rn.f32.s32 %0, %1;"
+                             : "=f"(v[r][i])
+                             : "r"(__float_as_int(v[r][i]) - kBias));
+    }
+}
+
+// 32 sums scaled: v = v * s * t + b (b null: no bias).
 __device__ __forceinline__ void scale32(float (&v)[32], float s, const float *t, const float *b) {
     const float2 s2 = make_float2(s, s);
 #pragma unroll
@@ -207,12 +257,8 @@ __device__ __forceinline__ void scale32(float (&v)[32], float s, const float *t,
         const float4 tv = reinterpret_cast<const float4 *>(t)[i];
         float4 bv = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (b) bv = reinterpret_cast<const float4 *>(b)[i];
-        const float2 a0 = mul_f32x2(make_float2((float)__float_as_int(v[4 * i]),
-                                                (float)__float_as_int(v[4 * i + 1])),
-                                    s2);
-        const float2 a1 = mul_f32x2(make_float2((float)__float_as_int(v[4 * i + 2]),
-                                                (float)__float_as_int(v[4 * i + 3])),
-                                    s2);
+        const float2 a0 = mul_f32x2(make_float2(v[4 * i], v[4 * i + 1]), s2);
+        const float2 a1 = mul_f32x2(make_float2(v[4 * i + 2], v[4 * i + 3]), s2);
         const float2 r0 = fma_f32x2(a0, make_float2(tv.x, tv.y), make_float2(bv.x, bv.y));
         const float2 r1 = fma_f32x2(a1, make_float2(tv.z, tv.w), make_float2(bv.z, bv.w));
         v[4 * i] = r0.x;
@@ -222,21 +268,21 @@ __device__ __forceinline__ void scale32(float (&v)[32], float s, const float *t,
     }
 }
 
-__device__ __forceinline__ void act32(float (&v)[32], int act, bool f32) {
-    if (act == kI8None) return;
-    if (f32) {
+template <typename F>
+__device__ __forceinline__ void pairs(float (&v)[32], F f) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = i8::act_full(v[i], act);
-    } else if (act == kI8Silu) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = epi::silu_fast(v[i]);
-    } else if (act == kI8GeluErf) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = i8::gelu_erf_16(v[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = epi::gelu_tanh_fast(v[i]);
+    for (int i = 0; i < 16; ++i) {
+        const float2 r = f(make_float2(v[2 * i], v[2 * i + 1]));
+        v[2 * i] = r.x;
+        v[2 * i + 1] = r.y;
     }
+}
+
+__device__ __forceinline__ void act32(float (&v)[32], int act) {
+    if (act == kI8None) return;
+    if (act == kI8Silu) pairs(v, i8::silu);
+    else if (act == kI8GeluErf) pairs(v, i8::gelu_erf);
+    else pairs(v, i8::gelu_tanh);
 }
 
 // Whole row segments from registers: N values at y + off (16-bit: packed).
@@ -256,11 +302,9 @@ __device__ __forceinline__ void store_row(const I8Params &p, size_t off, const f
         }
         return;
     }
-    const bool f16 = p.type == kI8F16;
     uint16_t *o = static_cast<uint16_t *>(p.y) + off;
     uint32_t w[N / 2];
-#pragma unroll
-    for (int i = 0; i < N / 2; ++i) w[i] = pack16x2(v[2 * i], v[2 * i + 1], f16);
+    pack32(w, v, p.type == kI8F16);
     const uintptr_t at = reinterpret_cast<uintptr_t>(o);
     if ((at & 31) == 0) {
 #pragma unroll
@@ -283,48 +327,61 @@ __device__ __forceinline__ void store_row(const I8Params &p, size_t off, const f
     }
 }
 
-// One 128-row x BN accumulator.  cols: this warpgroup's scales [BN] then biases [BN].
-template <int BN, int EPI>
+// Column of the tile's accumulator behind entry j of a warpgroup's column table
+// (its units of 32 columns, gate and up for the gated form, or its heads).
+template <int BN, int EPI, int HD, int G>
+__device__ __forceinline__ int table_col(int g, int j) {
+    if (EPI == kI8Store) return (g + j / 32 * G) * 32 + j % 32;
+    if (EPI == kI8Gated) return j / 32 % 2 * (BN / 2) + (g + j / 64 * G) * 32 + j % 32;
+    return (g + j / (HD ? HD : 1) * G) * HD + j % (HD ? HD : 1);
+}
+
+// One 128-row x BN accumulator; a warpgroup takes every G-th unit of 32 output
+// columns.  cols: the scales, then (NC on) the biases of its columns.  release
+// is called once the accumulator has been read.
+template <int BN, int EPI, int G, int NC, typename F>
 __device__ __forceinline__ void epilogue(const I8Params &p, uint32_t tbase, float s, int nb, int g,
-                                         const float *cols, Sink &sink) {
-    const bool f32 = p.type == kI8F32;
-    const float *bias = p.bias ? cols + BN : nullptr;
+                                         const float *cols, Sink &sink, F release) {
+    const float *bias = p.bias ? cols + NC : nullptr;
     if constexpr (EPI == kI8Store) {
-        // Two units of 32 columns per TMEM round trip.
-        constexpr int UNITS = BN / 32 / kGroups;
+        constexpr int UNITS = NC / 32;
 #pragma unroll 1
-        for (int u = 0; u < UNITS; u += 2) {
-            const int c0 = (g * UNITS + u) * 32;
-            if (nb * BN + c0 >= p.N) break;
-            float v[32], w[32];
-            tmem_ld32(tbase + c0, v);
-            if (UNITS > 1) tmem_ld32(tbase + c0 + 32, w);
-            tmem_wait_ld();
-            scale32(v, s, cols + c0, bias ? bias + c0 : nullptr);
-            act32(v, p.act, f32);
-            sink.put(v, nb * BN + c0);
-            if (UNITS > 1 && nb * BN + c0 + 32 < p.N) {
-                scale32(w, s, cols + c0 + 32, bias ? bias + c0 + 32 : nullptr);
-                act32(w, p.act, f32);
-                sink.put(w, nb * BN + c0 + 32);
+        for (int u = 0; u < UNITS; ++u) {
+            const int c = (g + u * G) * 32;
+            const bool in = c < BN && nb * BN + c < p.N;
+            float v[1][32];
+            if (in) {
+                tmem_ld32(tbase + c, v[0]);
+                tmem_wait_ld();
             }
+            if (u == UNITS - 1) release();
+            if (!in) continue;
+            to_f32(v);
+            scale32(v[0], s, cols + u * 32, bias ? bias + u * 32 : nullptr);
+            act32(v[0], p.act);
+            sink.put(v[0], nb * BN + c);
         }
     } else {
-        const float *bias2 = p.bias2 ? cols + BN + BN / 2 : nullptr;
+        constexpr int UNITS = NC / 64;
 #pragma unroll 1
-        for (int c = g; c < BN / 64; c += kGroups) {
-            const int col = nb * (BN / 2) + c * 32;
-            if (col >= p.N) break;
-            float a[32], u[32];
-            tmem_ld32(tbase + c * 32, a);
-            tmem_ld32(tbase + BN / 2 + c * 32, u);
-            tmem_wait_ld();
-            scale32(a, s, cols + c * 32, bias ? bias + c * 32 : nullptr);
-            scale32(u, s, cols + BN / 2 + c * 32, bias2 ? bias2 + c * 32 : nullptr);
-            act32(a, p.act, f32);
+        for (int k = 0; k < UNITS; ++k) {
+            const int c = (g + k * G) * 32, col = nb * (BN / 2) + c;
+            const bool in = c < BN / 2 && col < p.N;
+            float v[2][32];  // gate, up
+            if (in) {
+                tmem_ld32(tbase + c, v[0]);
+                tmem_ld32(tbase + BN / 2 + c, v[1]);
+                tmem_wait_ld();
+            }
+            if (k == UNITS - 1) release();
+            if (!in) continue;
+            to_f32(v);
+            scale32(v[0], s, cols + k * 64, bias ? bias + k * 64 : nullptr);
+            act32(v[0], p.act);
+            scale32(v[1], s, cols + k * 64 + 32, p.bias2 ? cols + NC + k * 64 + 32 : nullptr);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) a[i] *= u[i];
-            sink.put(a, col);
+            for (int i = 0; i < 32; ++i) v[0][i] *= v[1][i];
+            sink.put(v[0], col);
         }
     }
 }
@@ -332,14 +389,18 @@ __device__ __forceinline__ void epilogue(const I8Params &p, uint32_t tbase, floa
 // The head form: a warpgroup takes every second head of the tile.  A thread
 // holds its row's whole head in registers, so TMEM is read once.  rope: the
 // row's cos and sin [HD / 2] each (shared memory); norms: q_norm, k_norm [HD].
-template <int BN, int HD>
+template <int BN, int HD, int G, int NC, typename F>
 __device__ __forceinline__ void epilogue_heads(const I8Params &p, uint32_t tbase, int grow, float s,
                                                bool bad, int nb, int g, const float *cols,
-                                               const float *rope, const float *norms) {
+                                               const float *rope, const float *norms, F release) {
     constexpr int HALF = HD / 2, H32 = HALF / 32;
-    const float *bias = p.bias ? cols + BN : nullptr;
+    const float *bias = p.bias ? cols + NC : nullptr;
+    if (g * HD >= BN || nb * BN + g * HD >= p.N) {
+        release();
+        return;
+    }
 #pragma unroll 1
-    for (int h0 = g * HD; h0 < BN; h0 += kGroups * HD) {
+    for (int h0 = g * HD, k = 0; h0 < BN; h0 += G * HD, ++k) {
         const int col0 = nb * BN + h0;
         if (col0 >= p.N) break;
         const int head = col0 / HD;
@@ -350,9 +411,14 @@ __device__ __forceinline__ void epilogue_heads(const I8Params &p, uint32_t tbase
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c) tmem_ld32(tbase + h0 + c * 32, v[c]);
         tmem_wait_ld();
+        if (h0 + G * HD >= BN || col0 + G * HD >= p.N) release();  // the last head
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c)
-            scale32(v[c], s, cols + h0 + c * 32, bias ? bias + h0 + c * 32 : nullptr);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[c][i] = (float)__float_as_int(v[c][i]);
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c)
+            scale32(v[c], s, cols + k * HD + c * 32, bias ? bias + k * HD + c * 32 : nullptr);
         if (rot) {
             const bool normed = is_q ? p.q_norm != nullptr : p.k_norm != nullptr;
             float inv = bad ? i8::nan_f() : 1.0f;
@@ -450,13 +516,13 @@ struct Tiles {
 };
 
 template <int BN, int EPI, int HD>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Cfg<BN, EPI, HD>::THREADS), 1)
     i8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmB2,
                    const __grid_constant__ CUtensorMap tmOut, const I8Params p, const int tma_out) {
     extern __shared__ uint8_t smem_raw[];
     using CF = Cfg<BN, EPI, HD>;
-    constexpr int STAGES = CF::STAGES;
+    constexpr int STAGES = CF::STAGES, GROUPS = CF::GROUPS;
     __shared__ __align__(8) uint64_t full_bar[STAGES];
     __shared__ __align__(8) uint64_t empty_bar[STAGES];
     __shared__ __align__(8) uint64_t tfull_bar[2];
@@ -488,7 +554,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(&tfull_bar[a], 1);
-            mbar_init(&tempty_bar[a], 2 * 4 * kGroups);
+            mbar_init(&tempty_bar[a], 2 * 4 * GROUPS);
         }
         mbar_init(&drain_bar, 1);
         abort_sh = 0;
@@ -598,45 +664,68 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int row = q * 32 + lane;
         const int gt = (warp - 2 - 4 * g) * 32 + lane;  // thread of the warpgroup
         const int et = (warp - 2) * 32 + lane;          // thread of the epilogue
-        float *cols0 = reinterpret_cast<float *>(smem + CF::OFF_COLS) + g * 4 * BN;
-        Sink sink{p, &tmOut, smem + CF::OFF_STAGING + (warp - 2) * 2 * CHUNK, lane, 0, tma_out != 0};
+        constexpr int NC = CF::GCOLS, LOADS = (2 * NC + 127) / 128;
+        float *cols0 = reinterpret_cast<float *>(smem + CF::OFF_COLS) + g * 4 * NC;
+        Sink sink{p, &tmOut, smem + CF::OFF_STAGING + (warp - 2) * CHUNK, lane, 0, tma_out != 0};
         float *rope = reinterpret_cast<float *>(smem + CF::OFF_STAGING);
         float *norms = reinterpret_cast<float *>(smem + CF::OFF_NORMS);
         if (EPI == kI8Heads) {
-            for (int i = et; i < HD; i += 128 * kGroups) {
+            for (int i = et; i < HD; i += 128 * GROUPS) {
                 norms[i] = p.q_norm ? __ldg(p.q_norm + i) : 1.0f;
                 norms[HD + i] = p.k_norm ? __ldg(p.k_norm + i) : 1.0f;
             }
         }
-        int lt = 0, mb, nb, rope_mb = -1;
-        bool bad = false;
-        for (; tiles.pop(mb, nb); ++lt) {
-            const int a = lt & 1;
-            const uint32_t aph = (lt >> 1) & 1;
-            const int y0 = mb * 2 * BM + (int)rank * BM;
-            const int grow = y0 + row;
-            // Fetched while the tile's products run: the row's scale, the
-            // columns' scales and biases (in turns of two buffers: a thread
-            // passes the barrier below only after the tile before last).
-            const float s = grow < p.M ? __ldg(p.xs + grow) : 0.0f;
-            float *cols = cols0 + a * 2 * BN;
-            for (int c = gt; c < BN; c += 128) {
+        // A tile's row scale, column scales and biases are fetched one tile
+        // ahead; the columns' go through two buffers in shared memory (a thread
+        // writes one after a barrier that all of its last readers have passed).
+        float s_next = 0.0f, c_next[LOADS];
+        auto fetch = [&](int mb, int nb) {
+            const int grow = mb * 2 * BM + (int)rank * BM + row;
+            s_next = grow < p.M ? __ldg(p.xs + grow) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int e = gt + i * 128;
+                c_next[i] = 0.0f;
+                if (e >= 2 * NC) break;
+                const int c = table_col<BN, EPI, HD, GROUPS>(g, e % NC);
                 const bool second = EPI == kI8Gated && c >= TN;
                 const int col = nb * TN + (second ? c - TN : c);
-                const float *t = second ? p.ws2 : p.ws, *b = second ? p.bias2 : p.bias;
-                cols[c] = col < p.N ? __ldg(t + col) : 0.0f;
-                cols[BN + c] = b && col < p.N ? __ldg(b + col) : 0.0f;
+                const float *src = e < NC ? (second ? p.ws2 : p.ws) : (second ? p.bias2 : p.bias);
+                if (src && c < BN && col < p.N) c_next[i] = __ldg(src + col);
             }
+        };
+        auto keep = [&](float *cols) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i)
+                if (gt + i * 128 < 2 * NC) cols[gt + i * 128] = c_next[i];
+        };
+        int lt = 0, mb = 0, nb = 0, rope_mb = -1;
+        bool bad = false, more = tiles.pop(mb, nb);
+        if (more) {
+            fetch(mb, nb);
+            keep(cols0);
+        }
+        for (; more; ++lt) {
+            const int a = lt & 1;
+            const uint32_t aph = (lt >> 1) & 1;
+            const int mb0 = mb, nb0 = nb;
+            const int y0 = mb0 * 2 * BM + (int)rank * BM;
+            const int grow = y0 + row;
+            const float s = s_next;
+            float *cols = cols0 + a * 2 * NC;
+            more = tiles.pop(mb, nb);
+            if (more) fetch(mb, nb);
             if constexpr (EPI == kI8Heads) {
-                if (mb != rope_mb) {
+                if (mb0 != rope_mb) {
                     // The rotary rows of this row block: a warp copies 16 rows,
                     // one at a time.  All warps are past their last reads.
-                    rope_mb = mb;
-                    named_bar(1 + kGroups, 128 * kGroups);
+                    rope_mb = mb0;
+                    named_bar(1 + GROUPS, 128 * GROUPS);
                     const int ps = grow < p.M ? __ldg(p.pos + grow) : 0;
                     bad = ps < 0 || ps >= p.n_pos;
                     if (bad) set_error(p.err, kErrBadPosition);
                     constexpr int V = HD / 4;  // float4 per row, cos then sin
+#pragma unroll 8
                     for (int i = 0; i < 16; ++i) {
                         const int r = q * 32 + g * 16 + i;
                         int rp = __shfl_sync(0xffffffffu, ps, g * 16 + i);
@@ -647,28 +736,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                 __ldg(reinterpret_cast<const float4 *>(src) + lane % (V / 2));
                         }
                     }
-                    named_bar(1 + kGroups, 128 * kGroups);
+                    named_bar(1 + GROUPS, 128 * GROUPS);
                 }
             }
             // One verdict for the warpgroup (its barriers need all of it), and
             // in the head form for both.
             const bool ok = mbar_wait(&tfull_bar[a], aph, p.err, &abort_sh);
-            if (!(EPI == kI8Heads ? named_bar_and(1 + kGroups, 128 * kGroups, ok)
+            if (!(EPI == kI8Heads ? named_bar_and(1 + GROUPS, 128 * GROUPS, ok)
                                   : named_bar_and(1 + g, 128, ok)))
                 break;
             tc_fence_after();
             const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + a * BN;
+            auto release = [&]() {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_leader(&tempty_bar[a]);
+            };
             sink.y0 = y0 + q * 32;
-            if constexpr (EPI == kI8Heads) {
-                if (y0 < p.M)
-                    epilogue_heads<BN, HD>(p, tbase, grow, s, bad, nb, g, cols,
-                                           rope + row * CF::ROPE_LD, norms);
-            } else {
-                if (sink.y0 < p.M) epilogue<BN, EPI>(p, tbase, s, nb, g, cols, sink);
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_leader(&tempty_bar[a]);
+            if (sink.y0 >= p.M)
+                release();
+            else if constexpr (EPI == kI8Heads)
+                epilogue_heads<BN, HD, GROUPS, NC>(p, tbase, grow, s, bad, nb0, g, cols,
+                                                   rope + row * CF::ROPE_LD, norms, release);
+            else
+                epilogue<BN, EPI, GROUPS, NC>(p, tbase, s, nb0, g, cols, sink, release);
+            if (more) keep(cols0 + (a ^ 1) * 2 * NC);
         }
         if (EPI != kI8Heads) sink.finish();
     }
@@ -709,7 +801,7 @@ int launch(const I8Params &p, int num_sms, cudaStream_t stream) {
     constexpr int TN = EPI == kI8Gated ? BN / 2 : BN;
     const long long tiles = (long long)((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + TN - 1) / TN);
     const int grid = (int)std::min<long long>(2 * tiles, num_sms & ~1);
-    LAUNCH(launch_k(i8_gemm_kernel<BN, EPI, HD>, dim3(grid), dim3(kThreads), (Cfg<BN, EPI, HD>::SMEM), stream,
+    LAUNCH(launch_k(i8_gemm_kernel<BN, EPI, HD>, dim3(grid), dim3(Cfg<BN, EPI, HD>::THREADS), (Cfg<BN, EPI, HD>::SMEM), stream,
                     ma, mb, mb2, mo, p, tma ? 1 : 0));
     return 0;
 }

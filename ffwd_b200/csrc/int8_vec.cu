@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kWarps * 32) vec_store_kernel(const I8Params p
     const int n = n0 + lane / MT, m = lane % MT;
     if (lane < R * MT && n < p.N && m < p.M)
         i8::store1(p.y, p.type, (size_t)m * p.ldy + n,
-                   i8::act_full(scaled(a, __ldg(p.xs + m), p.ws, p.bias, n), p.act), p.accumulate);
+                   i8::act1(scaled(a, __ldg(p.xs + m), p.ws, p.bias, n), p.act), p.accumulate);
 }
 
 // R columns of gate and up each.
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kWarps * 32) vec_gated_kernel(const I8Params p
     const int n = n0 + lane / MT, m = lane % MT;
     if (lane < R * MT && n < p.N && m < p.M) {
         const float s = __ldg(p.xs + m);
-        const float g = i8::act_full(scaled(v, s, p.ws, p.bias, n), p.act);
+        const float g = i8::act1(scaled(v, s, p.ws, p.bias, n), p.act);
         i8::store1(p.y, p.type, (size_t)m * p.ldy + n, g * scaled(up, s, p.ws2, p.bias2, n), 0);
     }
 }
