@@ -4,20 +4,20 @@
 // per value.
 //
 // Rounding.  The code of a value is the nearest integer of v / s (s = amax / 127,
-// both quotients in f64; ties to even).  In f32 the
-// quotient is off by a few units in the last place (the product x * norm, the
-// reciprocal and the product with it: 4 x 2^-24 x 127 < 4e-5), which matters
-// only next to the border of two codes; there, about one value in 10^4, it is
-// taken again in f64.  The row's RMS cancels out of v / s, so with `norm` the
-// codes depend on x * norm alone and only the scale carries the RMS.
+// both quotients in f64; ties to even).  In f32 the quotient is off by a few
+// units in the last place, which matters only next to the border of two codes;
+// there it is taken again in f64: about one value in 10^5 of f32 rows, and of
+// bf16 rows one in 450, which lie on a border exactly.  The row's RMS cancels
+// out of v / s, so with `norm` the codes depend on x * norm alone and only the
+// scale carries the RMS.
 #include "int8.cuh"
 #include "launch_util.cuh"
 #include "ptx.cuh"
 
+#include <algorithm>
+
 namespace fb {
 namespace {
-
-constexpr float kTieBand = 4e-5f;
 
 template <int TYPE>
 __device__ __forceinline__ float load1(const void *x, size_t i) {
@@ -27,44 +27,82 @@ __device__ __forceinline__ float load1(const void *x, size_t i) {
     return __half2float(__ushort_as_half(h));
 }
 
-// Columns [c, c + 8) of the row at x; columns at or past K read as 0.
-template <int TYPE>
-__device__ __forceinline__ void load8(const void *x, size_t off, int c, int K, bool vec,
-                                      float (&v)[8]) {
-    if (vec && c + 8 <= K) {
-        if (TYPE == kI8F32) {
-            const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(x) + off + c);
-            const float4 a = __ldg(p), b = __ldg(p + 1);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(
-                static_cast<const uint16_t *>(x) + off + c));
-            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+// Eight values of a row as loaded, columns [c, c + 4) and [c + 128, c + 132):
+// a warp whose lanes are 4 columns apart reads 256 columns in whole lines, of
+// the row and of f32 norm weights alike.  16-bit types stay packed: half the
+// registers, so twice the rows in flight.
+template <int TYPE, bool VEC>
+struct Raw {
+    uint32_t w[TYPE == kI8F32 ? 8 : 4];
+
+    // Columns at or past K read as 0.  VEC: K and the addresses are multiples of
+    // four values.
+    __device__ __forceinline__ void load(const void *x, size_t off, int c, int K) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (TYPE == kI8BF16) {
-                    v[2 * i] = __uint_as_float(w[i] << 16);
-                    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        for (int h = 0; h < 2; ++h) {
+            const int ch = c + 128 * h;
+            if (TYPE == kI8F32) {
+                const uint32_t *p = static_cast<const uint32_t *>(x) + off + ch;
+                if (VEC) {
+                    uint4 r = make_uint4(0, 0, 0, 0);
+                    if (ch < K) r = __ldg(reinterpret_cast<const uint4 *>(p));
+                    w[4 * h] = r.x;
+                    w[4 * h + 1] = r.y;
+                    w[4 * h + 2] = r.z;
+                    w[4 * h + 3] = r.w;
                 } else {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-                    v[2 * i] = f.x;
-                    v[2 * i + 1] = f.y;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[4 * h + i] = ch + i < K ? p[i] : 0u;
+                }
+            } else {
+                const uint16_t *p = static_cast<const uint16_t *>(x) + off + ch;
+                if (VEC) {
+                    uint2 r = make_uint2(0, 0);
+                    if (ch < K) r = __ldg(reinterpret_cast<const uint2 *>(p));
+                    w[2 * h] = r.x;
+                    w[2 * h + 1] = r.y;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t lo = ch + 2 * i < K ? p[2 * i] : 0u;
+                        const uint32_t hi = ch + 2 * i + 1 < K ? p[2 * i + 1] : 0u;
+                        w[2 * h + i] = lo | hi << 16;
+                    }
                 }
             }
         }
-        return;
     }
+    __device__ __forceinline__ void unpack(float (&v)[8]) const {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < K ? load1<TYPE>(x, off + c + i) : 0.0f;
+        for (int i = 0; i < 4; ++i) {
+            if (TYPE == kI8F32) {
+                v[2 * i] = __uint_as_float(w[2 * i]);
+                v[2 * i + 1] = __uint_as_float(w[2 * i + 1]);
+            } else if (TYPE == kI8BF16) {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+            } else {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            }
+        }
+    }
+};
+
+template <bool VEC>
+__device__ __forceinline__ void load_norm(const float *w, int c, int K, float (&g)[8]) {
+    Raw<kI8F32, VEC> r;
+    r.load(w, 0, c, K);
+    r.unpack(g);
 }
 
-__device__ __forceinline__ void load8_norm(const float *w, int c, int K, bool vec, float (&g)[8]) {
-    load8<kI8F32>(w, 0, c, K, vec, g);
+// v / s in f64, correctly rounded, given rs = 1 / s to nearly f64's precision
+// (the quotient's first estimate and one correction from its exact remainder).
+__device__ __forceinline__ double quotient(double v, double s, double rs) {
+    const double t = v * rs;
+    return fma(fma(-t, s, v), rs, t);
 }
-
-// The residue of the f32 product x * w = p (exact unless it underflows).
-__device__ __forceinline__ float residue(float x, float w, float p) { return fmaf(x, w, -p); }
 
 // max(m, |v|), NaN if either is.
 __device__ __forceinline__ float max_abs(float m, float v) {
@@ -83,213 +121,238 @@ __device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d
     return __byte_perm(lo, hi, 0x5410);
 }
 
-// Codes of eight values (p = x, or x * g with a norm) of a row whose largest
-// magnitude is amax + amax_lo; written as 8 bytes, or as fewer at the row's end.
-template <bool NORM>
-__device__ __forceinline__ void put8(const float (&x)[8], const float (&g)[8], float inv,
-                                     float amax, float amax_lo, int8_t *q, int c, int K) {
-    float code[8];
+__device__ __forceinline__ float pick8(const float (&v)[8], int j) {
+    const float a = j & 1 ? v[1] : v[0], b = j & 1 ? v[3] : v[2];
+    const float c = j & 1 ? v[5] : v[4], d = j & 1 ? v[7] : v[6];
+    const float e = j & 2 ? b : a, f = j & 2 ? d : c;
+    return j & 4 ? f : e;
+}
+
+// Codes of eight values (x, or x * g with a norm) of a row whose largest
+// magnitude is amax + amax_lo, written at columns c and c + 128 on.  With SETTLE, values next to a border are settled; without, the result
+// says whether there are any.
+template <bool NORM, bool SETTLE, bool VEC>
+__device__ __forceinline__ bool put8(float (&x)[8], const float (&g)[8], float inv, float amax,
+                                     float amax_lo, int8_t *q, int c, int K) {
+    // How far the f32 quotient may be off: 127 x 2^-24 for the reciprocal's
+    // rounding; with a norm as much again for the product's and for amax's.
+    constexpr float kBand = NORM ? 2.6e-5f : 1e-5f;
+    float code[8], d[8];
     float far = 0.0f;  // largest distance from a code
     const float2 inv2 = make_float2(inv, inv), up = make_float2(kRound, kRound),
-                 down = make_float2(-kRound, -kRound);
+                 minus = make_float2(-1.0f, -1.0f);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         float2 t = make_float2(x[2 * i], x[2 * i + 1]);
         if (NORM) t = mul_f32x2(t, make_float2(g[2 * i], g[2 * i + 1]));
-        t = mul_f32x2(t, inv2);
-        const float2 f = add_f32x2(t, up);
-        const float2 d = add_f32x2(t, mul_f32x2(add_f32x2(f, down), make_float2(-1.0f, -1.0f)));
-        far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
+        const float2 f = fma_f32x2(t, inv2, up);
+        const float2 r = fma_f32x2(t, inv2, fma_f32x2(f, minus, up));
+        far = fmaxf(far, fmaxf(fabsf(r.x), fabsf(r.y)));
         code[2 * i] = f.x;
         code[2 * i + 1] = f.y;
+        d[2 * i] = r.x;
+        d[2 * i + 1] = r.y;
     }
     uint32_t w0 = low_bytes(code[0], code[1], code[2], code[3]);
     uint32_t w1 = low_bytes(code[4], code[5], code[6], code[7]);
-    if (far > 0.5f - kTieBand) {
-        // In f64, one value after another (a rare path, kept small).
-        const double s = ((double)amax + (double)amax_lo) / 127.0;
+    const bool any = far > 0.5f - kBand;
+    if (SETTLE && any) {
+        // In f64, one value after another (a rare path, kept small).  s = amax /
+        // 127 likewise; 1 / s from inv in two Newton steps.
+        const double am = (double)amax + (double)amax_lo;
+        const double s = quotient(am, 127.0, 1.0 / 127.0);
+        double rs = (double)inv;
+        rs = fma(fma(-s, rs, 1.0), rs, rs);
+        rs = fma(fma(-s, rs, 1.0), rs, rs);
         uint32_t near = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float d = (NORM ? x[i] * g[i] : x[i]) * inv - (code[i] - kRound);
-            near |= (fabsf(d) > 0.5f - 2.0f * kTieBand ? 1u : 0u) << i;
-        }
+        for (int i = 0; i < 8; ++i) near |= fabsf(d[i]) > 0.5f - kBand ? 1u << i : 0u;
 #pragma unroll 1
         for (; near; near &= near - 1) {
             const int j = __ffs(near) - 1;
-            float xj = x[0], gj = g[0];
-#pragma unroll
-            for (int i = 1; i < 8; ++i)
-                if (i == j) {
-                    xj = x[i];
-                    if (NORM) gj = g[i];
-                }
-            const double v = NORM ? (double)xj * (double)gj : (double)xj;
-            const uint32_t byte = (uint32_t)(int)rint(v / s) & 0xFF;
+            double v = (double)pick8(x, j);
+            if (NORM) v *= (double)pick8(g, j);
+            const uint32_t byte = (uint32_t)__double2int_rn(quotient(v, s, rs)) & 0xFF;
             const int sh = 8 * (j & 3);
             const uint32_t w = ((j < 4 ? w0 : w1) & ~(0xFFu << sh)) | byte << sh;
             if (j < 4) w0 = w;
             else w1 = w;
         }
     }
-    if (c + 8 <= K) {
-        *reinterpret_cast<uint2 *>(q + c) = make_uint2(w0, w1);
-    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (c + i < K) q[c + i] = (int8_t)((i < 4 ? w0 : w1) >> (8 * (i & 3)));
+    for (int h = 0; h < 2; ++h) {
+        const int ch = c + 128 * h;
+        const uint32_t w = h ? w1 : w0;
+        if (VEC) {
+            if (ch < K) *reinterpret_cast<uint32_t *>(q + ch) = w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (ch + i < K) q[ch + i] = (int8_t)(w >> (8 * i));
+        }
     }
+    return any;
+}
+
+// Blocks per SM that the registers allow: the row's values twice (this row's
+// and the next one's, in flight).
+constexpr int min_blocks(int type, bool norm, int w, int nv) {
+    const int regs = 48 + nv * (type == kI8F32 ? 16 : 8) + (norm ? 8 : 0);
+    const int n = 65536 / ((w > 8 ? w : 8) * 32 * regs);
+    return n < 1 ? 1 : n > 6 ? 6 : n;
 }
 
 // W warps per row, each thread holding NV groups of 8 columns (NV = 0: any
-// width, the row read again for the second pass).  A block of max(W, 8) warps.
-template <int TYPE, bool NORM, int W, int NV>
-__global__ void __launch_bounds__((W > 8 ? W : 8) * 32)
+// width, the row read again in each pass).  A block of max(W, 8) warps walks
+// over rows, the next row's loads in flight while it works on one.
+template <int TYPE, bool NORM, bool VEC, int W, int NV>
+__global__ void __launch_bounds__((W > 8 ? W : 8) * 32, min_blocks(TYPE, NORM, W, NV))
     quantize_kernel(const void *x, long long ldx, const float *norm, float eps, int8_t *q,
-                    long long ldq, float *s, int M, int K, int vec_x, int vec_n) {
-    constexpr int NW = W > 8 ? W : 8;
+                    long long ldq, float *s, int M, int K) {
+    constexpr int NW = W > 8 ? W : 8, R = NW / W;  // rows of a block at a time
     __shared__ uint32_t sh_max[NW];
     __shared__ float sh_sum[NW], sh_lo[NW];
     griddep_wait();
     griddep_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int wr = warp % W;  // warp of the row
-    const int row = blockIdx.x * (NW / W) + warp / W;
-    const bool live = row < M;
-    if (W == 1 && !live) return;
-    const size_t off = live ? (size_t)row * ldx : 0;
     const int t = wr * 32 + lane;
+    const int c0 = wr * 256 + lane * 4;  // first column of this thread's groups
     constexpr int NR = NV > 0 ? NV : 1;
-    float v[NR][8], g[NR][8];
-    float mv = 0.0f;
-    float ss = 0.0f;
-    auto stats = [&](const float(&a)[8], const float(&b)[8]) {
+    Raw<TYPE, VEC> next[NR];
+    auto prefetch = [&](int row) {
+        if (NV > 0 && row < M) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (NORM) ss = fmaf(a[i], a[i], ss);
-            mv = max_abs(mv, NORM ? a[i] * b[i] : a[i]);
+            for (int k = 0; k < NR; ++k)
+                next[k].load(x, (size_t)row * ldx, k * W * 256 + c0, K);
         }
     };
-    if (live) {
-        if (NV > 0) {
+    const int stride = gridDim.x * R;
+    prefetch(blockIdx.x * R + warp / W);
+    // (the block's rounds are counted by its first row: all of its warps take part)
+#pragma unroll 1
+    for (int row0 = blockIdx.x * R; row0 < M; row0 += stride) {
+        const int row = row0 + warp / W;
+        const bool live = row < M;
+        const size_t off = live ? (size_t)row * ldx : 0;
+        Raw<TYPE, VEC> raw[NR];
 #pragma unroll
-            for (int k = 0; k < NR; ++k) {
-                const int c = (k * W * 32 + t) * 8;
-                load8<TYPE>(x, off, c, K, vec_x, v[k]);
-                if (NORM) load8_norm(norm, c, K, vec_n, g[k]);
-            }
+        for (int k = 0; k < NR; ++k) raw[k] = next[k];
+        if (M - row0 > stride) prefetch(row + stride);
+        // Each of the passes over the row below: from registers, or loaded again.
+        auto each = [&](auto f) {
+            float v[8], g[8];
+            if (NV > 0) {
 #pragma unroll
-            for (int k = 0; k < NR; ++k) stats(v[k], g[k]);
-        } else {
-            for (int c = t * 8; c < K; c += W * 256) {
-                load8<TYPE>(x, off, c, K, vec_x, v[0]);
-                if (NORM) load8_norm(norm, c, K, vec_n, g[0]);
-                stats(v[0], g[0]);
-            }
-        }
-    }
-    // Magnitudes compare as unsigned integers, NaN above infinity.
-    const uint32_t mine = __float_as_uint(mv);
-    uint32_t mx = __reduce_max_sync(0xffffffffu, mine);
-    if (NORM) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    }
-    if (W > 1) {
-        if (lane == 0) {
-            sh_max[warp] = mx;
-            if (NORM) sh_sum[warp] = ss;
-        }
-        __syncthreads();
-        const int w0 = warp - wr;
-        mx = 0;
-        ss = 0.0f;
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-            mx = max(mx, sh_max[w0 + i]);
-            if (NORM) ss += sh_sum[w0 + i];
-        }
-    }
-    const float amax = __uint_as_float(mx);
-    float amax_lo = 0.0f;
-    if (NORM) {
-        // The largest product in full: among the values whose rounded product
-        // is the maximum, the largest residue (rounding keeps the order).
-        float lo = -INFINITY;
-        auto resid = [&](const float(&a)[8], const float(&b)[8]) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float p = a[i] * b[i];
-                if (fabsf(p) == amax) {
-                    const float e = residue(a[i], b[i], p);
-                    lo = fmaxf(lo, p < 0.0f ? -e : e);
+                for (int k = 0; k < NR; ++k) {
+                    const int c = k * W * 256 + c0;
+                    raw[k].unpack(v);
+                    if (NORM) load_norm<VEC>(norm, c, K, g);
+                    f(v, g, c);
+                }
+            } else {
+                for (int c = c0; c < K; c += W * 256) {
+                    raw[0].load(x, off, c, K);
+                    raw[0].unpack(v);
+                    if (NORM) load_norm<VEC>(norm, c, K, g);
+                    f(v, g, c);
                 }
             }
         };
-        if (live && mine == mx) {
-            if (NV > 0) {
+        float2 m2 = make_float2(0.0f, 0.0f), s2 = m2;
+        if (live)
+            each([&](const float(&a)[8], const float(&b)[8], int) {
 #pragma unroll
-                for (int k = 0; k < NR; ++k) resid(v[k], g[k]);
-            } else {
-                for (int c = t * 8; c < K; c += W * 256) {
-                    load8<TYPE>(x, off, c, K, vec_x, v[0]);
-                    load8_norm(norm, c, K, vec_n, g[0]);
-                    resid(v[0], g[0]);
+                for (int i = 0; i < 4; ++i) {
+                    float2 v = make_float2(a[2 * i], a[2 * i + 1]);
+                    if (NORM) {
+                        s2 = fma_f32x2(v, v, s2);
+                        v = mul_f32x2(v, make_float2(b[2 * i], b[2 * i + 1]));
+                    }
+                    m2.x = max_abs(m2.x, v.x);
+                    m2.y = max_abs(m2.y, v.y);
                 }
-            }
-        }
+            });
+        const float mv = max_abs(m2.x, m2.y);
+        float ss = s2.x + s2.y;
+        // Magnitudes compare as unsigned integers, NaN above infinity.
+        const uint32_t mine = __float_as_uint(mv);
+        uint32_t mx = __reduce_max_sync(0xffffffffu, mine);
+        if (NORM) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) lo = fmaxf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        }
         if (W > 1) {
-            if (lane == 0) sh_lo[warp] = lo;
+            __syncthreads();  // the last round's reads are done
+            if (lane == 0) {
+                sh_max[warp] = mx;
+                if (NORM) sh_sum[warp] = ss;
+            }
             __syncthreads();
             const int w0 = warp - wr;
-            lo = sh_lo[w0];
+            mx = 0;
+            ss = 0.0f;
 #pragma unroll
-            for (int i = 1; i < W; ++i) lo = fmaxf(lo, sh_lo[w0 + i]);
+            for (int i = 0; i < W; ++i) {
+                mx = max(mx, sh_max[w0 + i]);
+                if (NORM) ss += sh_sum[w0 + i];
+            }
         }
-        amax_lo = lo;
-    }
-    if (!live) return;
-    const bool finite = mx < 0x7F800000u && (!NORM || ss < INFINITY);
-    int8_t *qr = q + (size_t)row * ldq;
-    if (!finite || mx == 0) {
-        if (t == 0) s[row] = finite ? 0.0f : __uint_as_float(0x7FC00000u);
-        for (int c = t * 8; c < K; c += W * 256) {
-            if (c + 8 <= K)
-                *reinterpret_cast<uint2 *>(qr + c) = make_uint2(0, 0);
-            else
-                for (int i = c; i < K; ++i) qr[i] = 0;
+        const float amax = __uint_as_float(mx);
+        const bool finite = mx < 0x7F800000u && (!NORM || ss < INFINITY);
+        const bool plain = live && finite && amax >= 1e-30f;
+        int8_t *qr = q + (size_t)row * ldq;
+        if (live && t == 0)
+            s[row] = !finite ? __uint_as_float(0x7FC00000u)
+                     : NORM  ? amax / 127.0f / sqrtf(ss / (float)K + eps)
+                             : amax / 127.0f;
+        const float inv = 127.0f / amax;
+        bool open = false;  // codes left to settle
+        if (plain)
+            each([&](float(&a)[8], const float(&b)[8], int c) {
+                if (c < K) open |= put8<NORM, !NORM, VEC>(a, b, inv, amax, 0.0f, qr, c, K);
+            });
+        if (live && !plain) {
+            // 127 / amax may pass f32 for rows so small: a value at a time, in
+            // f64.  Rows of zeros, or not finite, get zeros.
+#pragma unroll 1
+            for (int c = t; c < K; c += W * 32) {
+                double v = (double)load1<TYPE>(x, off + c);
+                if (NORM) v *= (double)norm[c];
+                qr[c] = finite && amax > 0.0f ? (int8_t)(int)rint(v / ((double)amax / 127.0)) : 0;
+            }
         }
-        return;
-    }
-    if (t == 0) {
-        double sc = ((double)amax + (double)amax_lo) / 127.0;
-        if (NORM) sc /= sqrt((double)ss / (double)K + (double)eps);
-        s[row] = (float)sc;
-    }
-    if (amax < 1e-30f) {
-        // 127 / amax may pass f32: such rows go through f64, a value at a time.
-        const double sc = ((double)amax + (double)amax_lo) / 127.0;
-        for (int c = t; c < K; c += W * 32) {
-            double v = (double)load1<TYPE>(x, off + c);
-            if (NORM) v *= (double)norm[c];
-            qr[c] = (int8_t)(int)rint(v / sc);
-        }
-        return;
-    }
-    const float inv = 127.0f / amax;
-    if (NV > 0) {
+        if (NORM) {
+            // Settling takes the largest product in full: among the values whose
+            // rounded product is the maximum, the largest residue (rounding
+            // keeps the order).  Few rows need it.
+            if (!(W == 1 ? __any_sync(0xffffffffu, open) : __syncthreads_or(open))) continue;
+            float lo = -INFINITY;
+            if (plain && mine == mx)
+                each([&](const float(&a)[8], const float(&b)[8], int) {
 #pragma unroll
-        for (int k = 0; k < NR; ++k) {
-            const int c = (k * W * 32 + t) * 8;
-            if (c < K) put8<NORM>(v[k], g[k], inv, amax, amax_lo, qr, c, K);
-        }
-    } else {
-        for (int c = t * 8; c < K; c += W * 256) {
-            load8<TYPE>(x, off, c, K, vec_x, v[0]);
-            if (NORM) load8_norm(norm, c, K, vec_n, g[0]);
-            put8<NORM>(v[0], g[0], inv, amax, amax_lo, qr, c, K);
+                    for (int i = 0; i < 8; ++i) {
+                        const float p = a[i] * b[i];
+                        if (fabsf(p) == amax) {
+                            const float e = fmaf(a[i], b[i], -p);
+                            lo = fmaxf(lo, p < 0.0f ? -e : e);
+                        }
+                    }
+                });
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) lo = fmaxf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            if (W > 1) {
+                if (lane == 0) sh_lo[warp] = lo;
+                __syncthreads();
+                const int w0 = warp - wr;
+                lo = sh_lo[w0];
+#pragma unroll
+                for (int i = 1; i < W; ++i) lo = fmaxf(lo, sh_lo[w0 + i]);
+            }
+            if (open)
+                each([&](float(&a)[8], const float(&b)[8], int c) {
+                    if (c < K) put8<NORM, true, VEC>(a, b, inv, amax, lo, qr, c, K);
+                });
         }
     }
 }
@@ -302,34 +365,42 @@ struct Args {
     int8_t *q;
     long long ldq;
     float *s;
-    int M, K, vec_x, vec_n;
+    int M, K, num_sms;
 };
 
-template <int TYPE, bool NORM, int W, int NV>
+template <int TYPE, bool NORM, bool VEC, int W, int NV>
 cudaError_t run(const Args &a, cudaStream_t st) {
     constexpr int NW = W > 8 ? W : 8, R = NW / W;
-    return launch_k(quantize_kernel<TYPE, NORM, W, NV>, dim3((a.M + R - 1) / R), dim3(NW * 32), 0,
-                    st, a.x, a.ldx, a.norm, a.eps, a.q, a.ldq, a.s, a.M, a.K, a.vec_x, a.vec_n);
+    const int grid = std::min((a.M + R - 1) / R, a.num_sms * min_blocks(TYPE, NORM, W, NV));
+    return launch_k(quantize_kernel<TYPE, NORM, VEC, W, NV>, dim3(grid), dim3(NW * 32), 0, st, a.x,
+                    a.ldx, a.norm, a.eps, a.q, a.ldq, a.s, a.M, a.K);
 }
 
 // Many rows: as few warps per row as hold it (a warp's own reductions, no
 // block barrier).  Few rows (under two per SM): more warps per row, so that a
-// row's loads are all in flight at once.
+// row's loads are all in flight at once.  Columns or addresses that are no
+// multiple of four values: by element, the row read again in each pass.
 template <int TYPE, bool NORM>
-cudaError_t pick(const Args &a, bool few, cudaStream_t st) {
-    if (a.K <= 256) return run<TYPE, NORM, 1, 1>(a, st);
-    if (!few) {
-        if (a.K <= 512) return run<TYPE, NORM, 1, 2>(a, st);
-        if (a.K <= 1024) return run<TYPE, NORM, 1, 4>(a, st);
+cudaError_t pick(const Args &a, bool vec, cudaStream_t st) {
+    const bool few = a.M < 2 * a.num_sms;
+    if (!vec) {
+        return a.K <= 1024 && !few ? run<TYPE, NORM, false, 1, 0>(a, st)
+                                   : run<TYPE, NORM, false, 16, 0>(a, st);
     }
-    if (a.K <= 1024) return run<TYPE, NORM, 4, 1>(a, st);
+    if (a.K <= 256) return run<TYPE, NORM, true, 1, 1>(a, st);
     if (!few) {
-        if (a.K <= 2048) return run<TYPE, NORM, 4, 2>(a, st);
-        if (a.K <= 4096) return run<TYPE, NORM, 4, 4>(a, st);
+        if (a.K <= 512) return run<TYPE, NORM, true, 1, 2>(a, st);
+        if (a.K <= 1024) return run<TYPE, NORM, true, 1, 4>(a, st);
     }
-    if (a.K <= 4096) return run<TYPE, NORM, 16, 1>(a, st);
-    if (a.K <= 16384) return run<TYPE, NORM, 16, 4>(a, st);
-    return run<TYPE, NORM, 16, 0>(a, st);
+    if (a.K <= 1024) return run<TYPE, NORM, true, 4, 1>(a, st);
+    if (!few) {
+        if (a.K <= 2048) return run<TYPE, NORM, true, 4, 2>(a, st);
+        if (a.K <= 4096) return run<TYPE, NORM, true, 4, 4>(a, st);
+    }
+    if (a.K <= 4096) return run<TYPE, NORM, true, 16, 1>(a, st);
+    if (a.K <= 8192) return run<TYPE, NORM, true, 16, 2>(a, st);
+    if (a.K <= 16384) return run<TYPE, NORM, true, 16, 4>(a, st);
+    return run<TYPE, NORM, true, 16, 0>(a, st);
 }
 
 }  // namespace
@@ -337,16 +408,15 @@ cudaError_t pick(const Args &a, bool few, cudaStream_t st) {
 int i8_quantize_launch(const void *x, int type, long long ldx, const float *norm, float eps,
                        int8_t *q, long long ldq, float *s, int M, int K, int num_sms,
                        cudaStream_t stream) {
-    const int esz = type == kI8F32 ? 4 : 2;
-    const Args a{x, ldx, norm, eps, q, ldq, s, M, K,
-                 (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * esz) % 16 == 0,
-                 (reinterpret_cast<uintptr_t>(norm) & 15) == 0};
-    const bool few = M < 2 * num_sms;
+    const uintptr_t four = type == kI8F32 ? 16 : 8;  // bytes of four values
+    const bool vec = reinterpret_cast<uintptr_t>(x) % four == 0 && ldx % 4 == 0 && K % 4 == 0 &&
+                     reinterpret_cast<uintptr_t>(norm) % 16 == 0;
+    const Args a{x, ldx, norm, eps, q, ldq, s, M, K, num_sms};
     switch (type) {
-    case kI8F32: return norm ? pick<kI8F32, true>(a, few, stream) : pick<kI8F32, false>(a, few, stream);
+    case kI8F32: return norm ? pick<kI8F32, true>(a, vec, stream) : pick<kI8F32, false>(a, vec, stream);
     case kI8BF16:
-        return norm ? pick<kI8BF16, true>(a, few, stream) : pick<kI8BF16, false>(a, few, stream);
-    case kI8F16: return norm ? pick<kI8F16, true>(a, few, stream) : pick<kI8F16, false>(a, few, stream);
+        return norm ? pick<kI8BF16, true>(a, vec, stream) : pick<kI8BF16, false>(a, vec, stream);
+    case kI8F16: return norm ? pick<kI8F16, true>(a, vec, stream) : pick<kI8F16, false>(a, vec, stream);
     }
     return cudaErrorInvalidValue;
 }
