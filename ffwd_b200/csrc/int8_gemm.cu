@@ -28,10 +28,11 @@ constexpr int A_BYTES = BM * BK;
 constexpr int CHUNK = 2048;   // 32 rows x 64 bytes of output
 constexpr uint32_t kPeerMask = 0xFEFFFFFFu;  // clears the CTA-rank bit: leader's copy
 
-// Shared memory.  The head form keeps the rotary rows of the CTA's 128 rows
-// (cos and sin, f32, each row padded by 16 bytes so that 32 lanes reading 16
-// bytes of a row each meet no bank twice) and writes its heads straight from
-// registers; the others stage 2 KB of output per epilogue warp.  The head form
+// Shared memory: the stages, 2 KB of output per epilogue warp and, in the head
+// form, the rotary rows of the CTA's 128 rows (cos and sin, f32, each row
+// padded by 16 bytes so that 32 lanes reading 16 bytes of a row each meet no
+// bank twice).  Stores from registers would touch 32 rows an instruction (60
+// cycles of the shared-memory pipe each, 3000 a tile).  The head form
 // and the gated form have two epilogue warpgroups (a thread holds a whole head,
 // or 32 gate and 32 up sums), the plain one four.
 template <int BN, int EPI, int HD>
@@ -44,11 +45,11 @@ struct Cfg {
     static constexpr int GROUPS = EPI == kI8Store ? 4 : 2;  // epilogue warpgroups
     static constexpr int THREADS = 64 + 128 * GROUPS;
     static constexpr int ROPE_LD = HD + 4;  // floats
-    static constexpr int STAGING = HEADS ? BM * ROPE_LD * 4 : 4 * GROUPS * CHUNK;
+    static constexpr int OFF_ROPE = OFF_STAGING + 4 * GROUPS * CHUNK;
     // Per warpgroup, twice: the scales and biases of its columns of the tile.
     static constexpr int MIN_COLS = EPI == kI8Gated ? 64 : 32;  // of one unit
     static constexpr int GCOLS = HEADS ? 128 : BN / GROUPS < MIN_COLS ? MIN_COLS : BN / GROUPS;
-    static constexpr int OFF_COLS = OFF_STAGING + STAGING;
+    static constexpr int OFF_COLS = OFF_ROPE + (HEADS ? BM * ROPE_LD * 4 : 0);
     static constexpr int OFF_NORMS = OFF_COLS + GROUPS * 2 * 2 * GCOLS * 4;
     static constexpr int SMEM = OFF_NORMS + (HEADS ? 2 * HD * 4 : 0) + 1024;
     static constexpr int TMEM_COLS = 2 * BN;
@@ -285,48 +286,6 @@ __device__ __forceinline__ void act32(float (&v)[32], int act) {
     else pairs(v, i8::gelu_tanh);
 }
 
-// Whole row segments from registers: N values at y + off (16-bit: packed).
-// 32-byte stores where the address allows, else 16-byte ones, else elements.
-template <int N>
-__device__ __forceinline__ void store_row(const I8Params &p, size_t off, const float (&v)[N]) {
-    if (p.type == kI8F32) {
-        float *o = static_cast<float *>(p.y) + off;
-        if ((reinterpret_cast<uintptr_t>(o) & 15) == 0) {
-#pragma unroll
-            for (int i = 0; i < N / 4; ++i)
-                reinterpret_cast<float4 *>(o)[i] =
-                    make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) o[i] = v[i];
-        }
-        return;
-    }
-    uint16_t *o = static_cast<uint16_t *>(p.y) + off;
-    uint32_t w[N / 2];
-    pack32(w, v, p.type == kI8F16);
-    const uintptr_t at = reinterpret_cast<uintptr_t>(o);
-    if ((at & 31) == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 16; ++i)
-            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o + 16 * i),
-                         "r"(w[8 * i]), "r"(w[8 * i + 1]), "r"(w[8 * i + 2]), "r"(w[8 * i + 3]),
-                         "r"(w[8 * i + 4]), "r"(w[8 * i + 5]), "r"(w[8 * i + 6]), "r"(w[8 * i + 7])
-                         : "memory");
-    } else if ((at & 15) == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 8; ++i)
-            reinterpret_cast<uint4 *>(o)[i] =
-                make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) {
-            o[2 * i] = (uint16_t)w[i];
-            o[2 * i + 1] = (uint16_t)(w[i] >> 16);
-        }
-    }
-}
-
 // Column of the tile's accumulator behind entry j of a warpgroup's column table
 // (its units of 32 columns, gate and up for the gated form, or its heads).
 template <int BN, int EPI, int HD, int G>
@@ -390,9 +349,10 @@ __device__ __forceinline__ void epilogue(const I8Params &p, uint32_t tbase, floa
 // holds its row's whole head in registers, so TMEM is read once.  rope: the
 // row's cos and sin [HD / 2] each (shared memory); norms: q_norm, k_norm [HD].
 template <int BN, int HD, int G, int NC, typename F>
-__device__ __forceinline__ void epilogue_heads(const I8Params &p, uint32_t tbase, int grow, float s,
-                                               bool bad, int nb, int g, const float *cols,
-                                               const float *rope, const float *norms, F release) {
+__device__ __forceinline__ void epilogue_heads(const I8Params &p, uint32_t tbase, float s, bool bad,
+                                               int nb, int g, const float *cols,
+                                               const float *rope, const float *norms, Sink &sink,
+                                               F release) {
     constexpr int HALF = HD / 2, H32 = HALF / 32;
     const float *bias = p.bias ? cols + NC : nullptr;
     if (g * HD >= BN || nb * BN + g * HD >= p.N) {
@@ -406,7 +366,6 @@ __device__ __forceinline__ void epilogue_heads(const I8Params &p, uint32_t tbase
         const int head = col0 / HD;
         const bool is_q = head < p.n_q_heads;
         const bool rot = head < p.n_q_heads + p.n_kv_heads;
-        const size_t off = (size_t)grow * p.ldy + col0;
         float v[HD / 32][32];
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c) tmem_ld32(tbase + h0 + c * 32, v[c]);
@@ -437,40 +396,43 @@ __device__ __forceinline__ void epilogue_heads(const I8Params &p, uint32_t tbase
             const float *nw = norms + (is_q ? 0 : HD);
             const float2 inv2 = make_float2(inv, inv);
 #pragma unroll
-            for (int i = 0; i < HALF / 4; ++i) {
-                const float4 cv = reinterpret_cast<const float4 *>(rope)[i];
-                const float4 sv = reinterpret_cast<const float4 *>(rope + HALF)[i];
-                float4 w1 = make_float4(1.0f, 1.0f, 1.0f, 1.0f), w2 = w1;
-                if (normed) {
-                    w1 = reinterpret_cast<const float4 *>(nw)[i];
-                    w2 = reinterpret_cast<const float4 *>(nw + HALF)[i];
-                }
+            for (int c = 0; c < H32; ++c) {
+                float(&A)[32] = v[c], (&B)[32] = v[H32 + c];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int e = 4 * i + 2 * u;
-                    float(&A)[32] = v[e / 32], (&B)[32] = v[H32 + e / 32];
-                    const int j = e % 32;
-                    const float2 c2 = u ? make_float2(cv.z, cv.w) : make_float2(cv.x, cv.y);
-                    const float2 s2 = u ? make_float2(sv.z, sv.w) : make_float2(sv.x, sv.y);
-                    float2 a = mul_f32x2(make_float2(A[j], A[j + 1]), inv2);
-                    float2 b = mul_f32x2(make_float2(B[j], B[j + 1]), inv2);
+                for (int i = 0; i < 8; ++i) {
+                    const int e = c * 8 + i;
+                    const float4 cv = reinterpret_cast<const float4 *>(rope)[e];
+                    const float4 sv = reinterpret_cast<const float4 *>(rope + HALF)[e];
+                    float4 w1 = make_float4(1.0f, 1.0f, 1.0f, 1.0f), w2 = w1;
                     if (normed) {
-                        a = mul_f32x2(a, u ? make_float2(w1.z, w1.w) : make_float2(w1.x, w1.y));
-                        b = mul_f32x2(b, u ? make_float2(w2.z, w2.w) : make_float2(w2.x, w2.y));
+                        w1 = reinterpret_cast<const float4 *>(nw)[e];
+                        w2 = reinterpret_cast<const float4 *>(nw + HALF)[e];
                     }
-                    const float2 ns = make_float2(-s2.x, -s2.y);
-                    const float2 r1 = fma_f32x2(b, ns, mul_f32x2(a, c2));
-                    const float2 r2 = fma_f32x2(a, s2, mul_f32x2(b, c2));
-                    A[j] = r1.x;
-                    A[j + 1] = r1.y;
-                    B[j] = r2.x;
-                    B[j + 1] = r2.y;
-                }
-            }
-        }
-        if (grow < p.M) {
 #pragma unroll
-            for (int c = 0; c < HD / 32; ++c) store_row<32>(p, off + c * 32, v[c]);
+                    for (int u = 0; u < 2; ++u) {
+                        const int j = 4 * i + 2 * u;
+                        const float2 c2 = u ? make_float2(cv.z, cv.w) : make_float2(cv.x, cv.y);
+                        const float2 s2 = u ? make_float2(sv.z, sv.w) : make_float2(sv.x, sv.y);
+                        float2 a = mul_f32x2(make_float2(A[j], A[j + 1]), inv2);
+                        float2 b = mul_f32x2(make_float2(B[j], B[j + 1]), inv2);
+                        if (normed) {
+                            a = mul_f32x2(a, u ? make_float2(w1.z, w1.w) : make_float2(w1.x, w1.y));
+                            b = mul_f32x2(b, u ? make_float2(w2.z, w2.w) : make_float2(w2.x, w2.y));
+                        }
+                        const float2 r1 = mul_f32x2(a, c2);
+                        const float2 r2 = fma_f32x2(a, s2, mul_f32x2(b, c2));
+                        A[j] = fmaf(-b.x, s2.x, r1.x);
+                        A[j + 1] = fmaf(-b.y, s2.y, r1.y);
+                        B[j] = r2.x;
+                        B[j + 1] = r2.y;
+                    }
+                }
+                sink.put(A, col0 + c * 32);
+                sink.put(B, col0 + HALF + c * 32);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) sink.put(v[c], col0 + c * 32);
         }
     }
 }
@@ -667,7 +629,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Cfg<BN, EPI, HD>::T
         constexpr int NC = CF::GCOLS, LOADS = (2 * NC + 127) / 128;
         float *cols0 = reinterpret_cast<float *>(smem + CF::OFF_COLS) + g * 4 * NC;
         Sink sink{p, &tmOut, smem + CF::OFF_STAGING + (warp - 2) * CHUNK, lane, 0, tma_out != 0};
-        float *rope = reinterpret_cast<float *>(smem + CF::OFF_STAGING);
+        float *rope = reinterpret_cast<float *>(smem + CF::OFF_ROPE);
         float *norms = reinterpret_cast<float *>(smem + CF::OFF_NORMS);
         if (EPI == kI8Heads) {
             for (int i = et; i < HD; i += 128 * GROUPS) {
@@ -756,13 +718,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Cfg<BN, EPI, HD>::T
             if (sink.y0 >= p.M)
                 release();
             else if constexpr (EPI == kI8Heads)
-                epilogue_heads<BN, HD, GROUPS, NC>(p, tbase, grow, s, bad, nb0, g, cols,
-                                                   rope + row * CF::ROPE_LD, norms, release);
+                epilogue_heads<BN, HD, GROUPS, NC>(p, tbase, s, bad, nb0, g, cols,
+                                                   rope + row * CF::ROPE_LD, norms, sink, release);
             else
                 epilogue<BN, EPI, GROUPS, NC>(p, tbase, s, nb0, g, cols, sink, release);
             if (more) keep(cols0 + (a ^ 1) * 2 * NC);
         }
-        if (EPI != kI8Heads) sink.finish();
+        sink.finish();
     }
 
     tc_fence_before();
@@ -788,8 +750,7 @@ int launch(const I8Params &p, int num_sms, cudaStream_t stream) {
     if (EPI == kI8Gated && make_map_ld(&mb2, p.w2, p.N, p.K, p.ldw2, BN / 2, BK, SW, U8, 1))
         return -1;
     const int esz = p.type == kI8F32 ? 4 : 2;
-    const bool tma = EPI != kI8Heads && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 &&
-                     (p.ldy * esz) % 16 == 0;
+    const bool tma = (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && (p.ldy * esz) % 16 == 0;
     mo = ma;
     if (tma && make_map_ld(&mo, p.y, p.M, p.N, p.ldy, 32, 64 / esz, CU_TENSOR_MAP_SWIZZLE_64B,
                            p.type == kI8F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
