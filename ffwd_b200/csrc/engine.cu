@@ -12,6 +12,7 @@
 #include "attention.cuh"
 #include "gemm.cuh"
 #include "host_util.h"
+#include "int8.cuh"
 #include "loader.h"
 #include "ptx.cuh"
 #include "late.cuh"
@@ -43,6 +44,7 @@ namespace {
 
 int g_gemm_mode = 0;         // 0 f32, 1 tf32, 2 bf16, 3 16f (reference default: f32)
 int g_weight_override = -1;  // -1 file dtype, 0 f32, 1 bf16, 2 f16
+bool g_linear_i8 = false;    // projections in 8-bit integers (16-bit plans)
 std::vector<int> g_devices;
 bool g_devices_set = false;
 int g_max_tokens = 262144;
@@ -160,6 +162,10 @@ struct Mat {
     int rows = 0, cols = 0, bn = 128;
     CUtensorMap map_hi, map_lo;
     CUtensorMap map_half;  // 128-row box over hi, for the two-SM kernel (bn == 256)
+    // 8-bit plan, instead of the above: codes [rows, cols] and a scale per row
+    // (a fused gate / up pair: gate rows, then up rows).
+    int8_t *q8 = nullptr;
+    float *scale = nullptr;
 };
 
 struct LayerW {
@@ -180,6 +186,10 @@ struct Workspace {
     __nv_bfloat16 *xb = nullptr, *xb_lo = nullptr;
     void *qkv = nullptr;
     __nv_bfloat16 *att = nullptr, *att_lo = nullptr, *hmid = nullptr, *hmid_lo = nullptr;
+    // 8-bit plan: the next projection's quantised rows (the widest one's) and
+    // their scales.
+    int8_t *q8 = nullptr;
+    float *q8_scale = nullptr;
     // pinned host staging
     int *h_ids = nullptr, *h_offsets = nullptr, *h_err = nullptr, *h_spans = nullptr;
     AttnItem *h_items = nullptr;
@@ -250,6 +260,7 @@ struct ffwd_b200_ctx {
     ffwd_config_t cfg;
     int prec = 0;      // 0 single pass, 2 / 3 split-bf16 passes, 4 kind::tf32
     bool f16 = false;  // single-pass operands in f16 (else bf16)
+    bool i8 = false;   // projections in 8-bit integers (prec 0: attention stays 16-bit)
     std::vector<fb::Device> devs;
     float lin_flops_per_token = 0.0f;
     int token_dim = 0;  // late interaction: 1_Dense output width (0: pooled model)
@@ -294,6 +305,8 @@ int upload(Device &D, T **p, const std::vector<T> &h) {
 struct HostMat {
     std::vector<uint16_t> hi, lo;
     std::vector<float> f32;  // tf32 plan: f32 values rounded to tf32
+    std::vector<int8_t> q8;  // 8-bit plan: codes, with a scale per row
+    std::vector<float> scale;
     int rows = 0, cols = 0;
 };
 
@@ -313,10 +326,10 @@ float round_tf32_host(float v) {
 // store: the device weight storage the values are first rounded to (0 f32,
 // 1 bf16, 2 f16; libffwd/cuda.cu upload_weight 262-305).  The encoding is then
 // f16 (out_f16, single-pass f16 GEMM), tf32-rounded f32 (out_tf32, kind::tf32
-// GEMM), or bf16 hi (+ lo = bf16(v - hi) when split).
+// GEMM), 8-bit codes with a scale per row (out_i8), or bf16 hi (+ lo = bf16(v - hi) when split).
 bool prep_mat(const std::vector<const TensorView *> &parts, const std::vector<std::string> &names,
-              int cols, int store, bool split, bool out_f16, bool out_tf32, int interleave,
-              HostMat &hm, std::string &err) {
+              int cols, int store, bool split, bool out_f16, bool out_tf32, bool out_i8,
+              int interleave, HostMat &hm, std::string &err) {
     int rows = 0;
     for (size_t i = 0; i < parts.size(); ++i) {
         const TensorView *t = parts[i];
@@ -328,7 +341,10 @@ bool prep_mat(const std::vector<const TensorView *> &parts, const std::vector<st
     }
     hm.rows = rows;
     hm.cols = cols;
-    if (out_tf32)
+    if (out_i8) {
+        hm.q8.resize((size_t)rows * cols);
+        hm.scale.resize(rows);
+    } else if (out_tf32)
         hm.f32.resize((size_t)rows * cols);
     else
         hm.hi.resize((size_t)rows * cols);
@@ -356,18 +372,35 @@ bool prep_mat(const std::vector<const TensorView *> &parts, const std::vector<st
         for (int r = r0; r < r1; ++r) {
             const TensorView *t = parts[src_part[r]];
             const size_t so = (size_t)src_row[r] * cols;
-            uint16_t *dh = out_tf32 ? nullptr : hm.hi.data() + (size_t)r * cols;
+            uint16_t *dh = out_tf32 || out_i8 ? nullptr : hm.hi.data() + (size_t)r * cols;
             uint16_t *dl = split ? hm.lo.data() + (size_t)r * cols : nullptr;
-            if (out_tf32) {
+            // Column c as f32, in the device weight storage's precision.
+            auto stored = [&](int c) {
+                float v = t->dtype == DType::F32    ? ((const float *)t->data)[so + c]
+                          : t->dtype == DType::BF16 ? bf16_to_f32(((const uint16_t *)t->data)[so + c])
+                                                    : f16_to_f32(((const uint16_t *)t->data)[so + c]);
+                if (store == 1) v = bf16_to_f32(f32_to_bf16_rne(v));
+                else if (store == 2) v = f16_to_f32(f32_to_f16_rne(v));
+                return v;
+            };
+            if (out_i8) {
+                // Nearest code of v / (amax / 127), as the row kernel rounds; a
+                // row that is not finite gets scale NaN and zeros.
+                float amax = 0.0f;
+                bool finite = true;
                 for (int c = 0; c < cols; ++c) {
-                    const uint16_t w = ((const uint16_t *)t->data)[so + c];
-                    float v = t->dtype == DType::F32    ? ((const float *)t->data)[so + c]
-                              : t->dtype == DType::BF16 ? bf16_to_f32(w)
-                                                        : f16_to_f32(w);
-                    if (store == 1) v = bf16_to_f32(f32_to_bf16_rne(v));
-                    else if (store == 2) v = f16_to_f32(f32_to_f16_rne(v));
-                    hm.f32[(size_t)r * cols + c] = round_tf32_host(v);
+                    const float v = stored(c);
+                    finite &= std::isfinite(v);
+                    amax = std::max(amax, std::fabs(v));
                 }
+                const double s = (double)amax / 127.0;
+                hm.scale[r] = finite ? amax / 127.0f : NAN;
+                for (int c = 0; c < cols; ++c)
+                    hm.q8[(size_t)r * cols + c] =
+                        finite && amax > 0.0f ? (int8_t)std::nearbyint((double)stored(c) / s) : 0;
+            } else if (out_tf32) {
+                for (int c = 0; c < cols; ++c)
+                    hm.f32[(size_t)r * cols + c] = round_tf32_host(stored(c));
             } else if (t->dtype == DType::BF16 && !out_f16 && store != 2) {
                 memcpy(dh, (const uint16_t *)t->data + so, (size_t)cols * 2);
             } else if (t->dtype == DType::F16 && out_f16) {
@@ -406,6 +439,7 @@ int upload_mat(Device &D, const HostMat &hm, int bn, Mat &m) {
     m.rows = hm.rows;
     m.cols = hm.cols;
     m.bn = bn;
+    if (!hm.q8.empty()) return upload(D, &m.q8, hm.q8) || upload(D, &m.scale, hm.scale) ? -1 : 0;
     if (!hm.f32.empty()) {  // tf32 plan: f32 weights, 32-column (128-byte) boxes
         float *d = nullptr;
         if (dev_alloc(D, &d, hm.f32.size())) return -1;
@@ -477,6 +511,7 @@ struct HostModel {
     int prec = 0;
     int store = 0;     // weight storage: 0 f32, 1 bf16, 2 f16
     bool f16 = false;  // single-pass operands are f16 (else bf16)
+    bool i8 = false;   // projections in 8-bit integers
     std::string prefix;
     SafeTensors st;
 };
@@ -505,8 +540,8 @@ int load_device(HostModel &hm, Device &D, std::string &err) {
         std::vector<const TensorView *> parts;
         for (auto &n : names) parts.push_back(T(n));
         HostMat h;
-        if (!prep_mat(parts, names, cols, hm.store, split_w, hm.f16, hm.prec == 4, interleave, h,
-                      err))
+        if (!prep_mat(parts, names, cols, hm.store, split_w, hm.f16, hm.prec == 4, hm.i8,
+                      hm.i8 ? 0 : interleave, h, err))
             return -1;
         return upload_mat(D, h, bn, m);
     };
@@ -621,7 +656,8 @@ void free_device(Device &D) {
     D.allocs.clear();
     Workspace &w = D.ws;
     void *dptrs[] = {w.ids, w.pos, w.offsets, w.err, w.span_starts, w.span_ends, w.items, w.pooled,
-                     w.x, w.xb, w.xb_lo, w.qkv, w.att, w.att_lo, w.hmid, w.hmid_lo, D.rope_cos,
+                     w.x, w.xb, w.xb_lo, w.qkv, w.att, w.att_lo, w.hmid, w.hmid_lo, w.q8,
+                     w.q8_scale, D.rope_cos,
                      D.rope_sin, D.rope_cos_h, D.rope_sin_h};
     for (void *q : dptrs)
         if (q) cudaFree(q);
@@ -671,6 +707,11 @@ int ws_free(T **p, bool host = false) {
     return 0;
 }
 
+// Columns of the widest projection input.
+size_t widest_rows(const ffwd_config_t &c) {
+    return std::max({c.hidden_size, c.q_dim, c.intermediate_size});
+}
+
 // Grow the workspace to T packed rows, B sequences, n_items attention items
 // and n_spans spans.  A capacity is set only once all of its buffers exist,
 // so a failed allocation leaves it at 0 and the next call allocates again.
@@ -686,7 +727,8 @@ int ensure_ws(ffwd_b200_ctx *ctx, Device &D, int T, int B, int n_items, int n_sp
         w.cap_t = 0;
         void **bufs[] = {(void **)&w.ids, (void **)&w.pos, (void **)&w.x, (void **)&w.xb,
                          (void **)&w.xb_lo, &w.qkv, (void **)&w.att, (void **)&w.att_lo,
-                         (void **)&w.hmid, (void **)&w.hmid_lo};
+                         (void **)&w.hmid, (void **)&w.hmid_lo, (void **)&w.q8,
+                         (void **)&w.q8_scale};
         for (void **b : bufs)
             if (ws_free(b)) return -1;
         if (ws_free(&w.h_ids, true)) return -1;
@@ -704,6 +746,10 @@ int ensure_ws(ffwd_b200_ctx *ctx, Device &D, int T, int B, int n_items, int n_sp
             CK(ws_malloc((void **)&w.xb_lo, t * H * 2));
             CK(ws_malloc((void **)&w.att_lo, t * c.q_dim * 2));
             CK(ws_malloc((void **)&w.hmid_lo, t * inter * 2));
+        }
+        if (ctx->i8) {
+            CK(ws_malloc((void **)&w.q8, t * widest_rows(c)));
+            CK(ws_malloc((void **)&w.q8_scale, t * 4));
         }
         CK(ws_malloc_host((void **)&w.h_ids, t * 4));
         w.cap_t = cap;
@@ -886,6 +932,15 @@ int setup_forward(ffwd_b200_ctx *ctx, Device &D, FwdState &fs, Workspace &w, int
     return embed_step(ctx, D, fs, w);
 }
 
+// Rows of the next 8-bit projection: x [T, K] of `type`, after an RMSNorm where
+// `norm` is given, to w.q8 and w.q8_scale.
+int quantize_rows(Device &D, Workspace &w, const void *x, int type, int T, int K, const float *norm,
+                  float eps) {
+    LAUNCH(i8_quantize_launch(x, type, K, norm, eps, w.q8, K, w.q8_scale, T, K, D.num_sms,
+                              D.stream));
+    return 0;
+}
+
 // Positions and the embedding (+ first norm) of the forward fs over w.
 int embed_step(ffwd_b200_ctx *ctx, Device &D, const FwdState &fs, Workspace &w) {
     const ffwd_config_t &c = ctx->cfg;
@@ -903,7 +958,9 @@ int embed_step(ffwd_b200_ctx *ctx, Device &D, const FwdState &fs, Workspace &w) 
                                D.type0, D.emb_ln_g, D.emb_ln_b, H, eps, w.x, xb_out, w.err, s));
     else
         LAUNCH(embed_rms_launch(w.ids, T, D.embed, D.embed_bf16, c.vocab_size, H, w.x,
-                                D.layers[0].in_norm, eps, xb_out, w.err, s));
+                                ctx->i8 ? nullptr : D.layers[0].in_norm, eps, xb_out, w.err, s));
+    if (ctx->i8)
+        return quantize_rows(D, w, w.x, kI8F32, T, H, bert ? nullptr : D.layers[0].in_norm, eps);
     return 0;
 }
 
@@ -938,6 +995,98 @@ int prepare(ffwd_b200_ctx *ctx, Device &D, FwdState &fs, int T, int B, const int
     return setup_forward(ctx, D, fs, w, T, B);
 }
 
+// The same ops with the projections in 8-bit integers.  Each projection reads
+// w.q8: the norms before QKV and FFN up quantise their rows as they write them
+// (the decoder's in one kernel), attention output and FFN activation are
+// quantised from their 16-bit buffers.
+int step_i8(ffwd_b200_ctx *ctx, Device &D, FwdState &fs, Workspace &w, int op, int li) {
+    const ffwd_config_t &c = ctx->cfg;
+    const int H = c.hidden_size, I = c.intermediate_size, T = fs.T;
+    const bool bert = c.family == FFWD_FAMILY_BERT;
+    const float eps = bert ? c.layer_norm_eps : c.rms_norm_eps;
+    const int type = ctx->f16 ? kI8F16 : kI8BF16;  // of qkv, attention and FFN activation
+    cudaStream_t s = D.stream;
+    const LayerW &l = D.layers[li];
+    auto product = [&](const Mat &m, int rows, const float *bias, void *y, int y_type) {
+        I8Params p{};
+        p.M = T;
+        p.N = rows;
+        p.K = m.cols;
+        p.x = w.q8;
+        p.ldx = m.cols;
+        p.xs = w.q8_scale;
+        p.w = m.q8;
+        p.ldw = m.cols;
+        p.ws = m.scale;
+        p.bias = bias;
+        p.y = y;
+        p.ldy = rows;
+        p.type = y_type;
+        p.err = w.err;
+        return p;
+    };
+    // LayerNorm of the residual stream (BERT), then its rows quantised; or the
+    // RMSNorm and quantisation in one.
+    auto norm = [&](const float *g, const float *b) {
+        if (bert) {
+            const RowOut xb{w.xb, nullptr, ctx->f16 ? 1 : 0, nullptr};
+            LAUNCH(layernorm_launch(w.x, T, H, g, b, eps, xb, s));
+        }
+        return quantize_rows(D, w, w.x, kI8F32, T, H, bert ? nullptr : g, eps);
+    };
+    switch (op) {
+    case kOpQKV: {
+        I8Params p = product(l.qkv, l.qkv.rows, l.b_qkv, w.qkv, type);
+        if (bert) return i8_project(kI8Store, p, D.num_sms, s);
+        p.pos = w.pos;
+        p.cos = D.rope_cos;
+        p.sin = D.rope_sin;
+        p.n_pos = D.rope_cap;
+        p.q_norm = l.q_norm;
+        p.k_norm = l.k_norm;
+        p.n_q_heads = c.n_heads;
+        p.n_kv_heads = c.n_kv_heads;
+        p.head_dim = c.head_dim;
+        p.eps = c.rms_norm_eps;
+        return i8_project(kI8Heads, p, D.num_sms, s);
+    }
+    case kOpAttn:
+        LAUNCH(attention_tc_launch(&fs.m_qkv, fs.ap, s));
+        return 0;
+    case kOpO: {
+        if (quantize_rows(D, w, w.att, type, T, c.q_dim, nullptr, eps)) return -1;
+        I8Params p = product(l.o, H, l.b_o, w.x, kI8F32);
+        p.accumulate = 1;
+        return i8_project(kI8Store, p, D.num_sms, s);
+    }
+    case kOpNorm1:
+        return norm(bert ? l.ln1_g : l.post_norm, l.ln1_b);
+    case kOpUp: {
+        I8Params p = product(l.up, I, l.b_up, w.hmid, type);
+        if (bert) {
+            p.act = c.ffn_act == FFWD_ACT_GELU_TANH ? kI8GeluTanh : kI8GeluErf;
+            return i8_project(kI8Store, p, D.num_sms, s);
+        }
+        p.act = kI8Silu;
+        p.w2 = l.up.q8 + (size_t)I * H;
+        p.ws2 = l.up.scale + I;
+        p.ldw2 = H;
+        return i8_project(kI8Gated, p, D.num_sms, s);
+    }
+    case kOpDown: {
+        if (quantize_rows(D, w, w.hmid, type, T, I, nullptr, eps)) return -1;
+        I8Params p = product(l.down, H, l.b_down, w.x, kI8F32);
+        p.accumulate = 1;
+        return i8_project(kI8Store, p, D.num_sms, s);
+    }
+    case kOpNorm2:
+        if (bert) return norm(l.ln2_g, l.ln2_b);
+        return li + 1 < c.n_layers ? norm(D.layers[li + 1].in_norm, nullptr) : 0;
+    }
+    fail("unknown op %d", op);
+    return -1;
+}
+
 // One op of layer li on the prepared forward.
 int step(ffwd_b200_ctx *ctx, Device &D, FwdState &fs, int op, int li) {
     const ffwd_config_t &c = ctx->cfg;
@@ -953,6 +1102,7 @@ int step(ffwd_b200_ctx *ctx, Device &D, FwdState &fs, int op, int li) {
     const LayerW &l = D.layers[li];
     const RowOut xb_out{w.xb, split ? w.xb_lo : nullptr, ctx->f16 ? 1 : 0,
                         ctx->prec == 4 ? reinterpret_cast<float *>(w.xb) : nullptr};
+    if (ctx->i8) return step_i8(ctx, D, fs, w, op, li);
     switch (op) {
     case kOpQKV: {  // QKV projection (+ bias, + QK-norm and RoPE on the decoder)
         GemmParams p{};
@@ -1309,6 +1459,11 @@ FFWD_B200_API int ffwd_b200_set_weights_default(void) {
     return 0;
 }
 
+FFWD_B200_API int ffwd_b200_set_linear_i8(int on) {
+    g_linear_i8 = on != 0;
+    return 0;
+}
+
 FFWD_B200_API int ffwd_b200_set_devices(const int *devices, int n) {
     if (n <= 0 || !devices) return -1;
     g_devices.assign(devices, devices + n);
@@ -1423,6 +1578,18 @@ ffwd_b200_ctx *load_ctx(const char *model_dir) {
         prec = 0;
         f16 = store == 2 || (store == 0 && g_gemm_mode == 3);
     }
+    if (g_linear_i8) {
+        if (prec != 0) {
+            fail("8-bit projections go with a 16-bit plan (--gpu-gemm-mode bf16 or 16f, or 16-bit "
+                 "decoder weights)");
+            return nullptr;
+        }
+        if (c.family != FFWD_FAMILY_BERT && c.head_dim == 32) {
+            fail("8-bit projections of a decoder need head_dim 64 or 128");
+            return nullptr;
+        }
+    }
+    hm->i8 = g_linear_i8;
     hm->prec = prec;
     hm->store = store;
     hm->f16 = f16;
@@ -1431,6 +1598,7 @@ ffwd_b200_ctx *load_ctx(const char *model_dir) {
     ctx->cfg = c;
     ctx->prec = prec;
     ctx->f16 = f16;
+    ctx->i8 = hm->i8;
     const int qkv_out = c.q_dim + 2 * c.kv_dim;
     ctx->lin_flops_per_token =
         2.0f * c.n_layers *
@@ -1480,7 +1648,9 @@ FFWD_B200_API const ffwd_config_t *ffwd_b200_config(const ffwd_b200_ctx_t *ctx) 
 }
 
 FFWD_B200_API int ffwd_b200_precision(const ffwd_b200_ctx_t *ctx) {
-    return ctx ? (ctx->prec == 0 && ctx->f16 ? 1 : ctx->prec) : -1;
+    if (!ctx) return -1;
+    if (ctx->i8) return 5;
+    return ctx->prec == 0 && ctx->f16 ? 1 : ctx->prec;
 }
 
 FFWD_B200_API int ffwd_b200_lpt_partition(const double *cost, int n, int n_parts, int *part) {
@@ -2321,6 +2491,8 @@ extern "C" FFWD_B200_API int ffwd_b200_encode_device_noalloc(ffwd_b200_ctx_t *ct
     if (ok && split)
         ok = cv.take(&w.xb_lo, (size_t)T * H) && cv.take(&w.att_lo, (size_t)T * c.q_dim) &&
              cv.take(&w.hmid_lo, (size_t)T * I);
+    if (ok && ctx->i8)
+        ok = cv.take(&w.q8, (size_t)T * widest_rows(c)) && cv.take(&w.q8_scale, (size_t)T);
     if (!ok) {
         fail("no-allocation encode: %d tokens need more than the %zu-byte scratch maximum", T,
              kNoAllocScratchBytes);

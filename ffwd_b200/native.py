@@ -79,6 +79,7 @@ ABI = {
     "ffwd_b200_set_weights_bf16": (ctypes.c_int, [ctypes.c_int]),
     "ffwd_b200_set_weights_f16": (ctypes.c_int, [ctypes.c_int]),
     "ffwd_b200_set_weights_default": (ctypes.c_int, []),
+    "ffwd_b200_set_linear_i8": (ctypes.c_int, [ctypes.c_int]),
     "ffwd_b200_load": (ctypes.c_void_p, [ctypes.c_char_p]),
     "ffwd_b200_free": (None, [ctypes.c_void_p]),
     "ffwd_b200_config": (ctypes.POINTER(ffwd_config_t), [ctypes.c_void_p]),
@@ -245,7 +246,8 @@ class B200Model:
     """One loaded model (the reference's ffwd_cuda_ctx_t)."""
 
     def __init__(self, model_dir: str, gemm_mode: str | None = None,
-                 weight_dtype: str | None = None, devices=None, max_tokens: int | None = None):
+                 weight_dtype: str | None = None, devices=None, max_tokens: int | None = None,
+                 linear_i8: bool = False):
         L = lib()
         if gemm_mode is not None and L.ffwd_b200_set_fast_gemm(gemm_mode.encode()) != 0:
             raise FfwdError("--gpu-gemm-mode must be f32, tf32, bf16, or 16f")
@@ -267,7 +269,9 @@ class B200Model:
         if max_tokens is not None:
             L.ffwd_b200_set_max_tokens(int(max_tokens))
         self._l = L
+        L.ffwd_b200_set_linear_i8(int(linear_i8))
         self.h = L.ffwd_b200_load(model_dir.encode())
+        L.ffwd_b200_set_linear_i8(0)
         if not self.h:
             raise FfwdError(f"failed to load model: {last_error()}")
         self.config = L.ffwd_b200_config(self.h).contents

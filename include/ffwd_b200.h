@@ -133,6 +133,14 @@ FFWD_B200_API int ffwd_b200_set_weights_f16(int on);
  * process). */
 FFWD_B200_API int ffwd_b200_set_weights_default(void);
 
+/* No reference counterpart.  With on = 1, the next loads run every projection of
+ * a layer in 8-bit integers (weights quantised with a scale per output channel
+ * as they are uploaded, activations with a scale per token as they are
+ * produced; exact 32-bit sums), with the plan's 16-bit attention and f32
+ * residual stream, norms and embedding: ffwd_b200_precision 5.  Goes with a
+ * 16-bit plan: loading with an exact or tf32 one is refused.  Default off. */
+FFWD_B200_API int ffwd_b200_set_linear_i8(int on);
+
 /* Load config + safetensors from model_dir and upload to every device of the
  * current device set.  Replaces ffwd_cuda_load (cuda.h:26; cuda.cu:4306). */
 FFWD_B200_API ffwd_b200_ctx_t *ffwd_b200_load(const char *model_dir);
@@ -299,7 +307,8 @@ FFWD_B200_API long long ffwd_b200_launch_count(void);
 FFWD_B200_API const char *ffwd_b200_last_error(void);
 /* Precision plan chosen at load: 0 = single-pass bf16, 1 = single-pass f16,
  * 2 = split-bf16 2-pass, 3 = split-bf16 3-pass, 4 = tf32 (kind::tf32 GEMMs over
- * tf32-rounded f32 operands, split-bf16 attention). */
+ * tf32-rounded f32 operands, split-bf16 attention), 5 = 8-bit integer
+ * projections, 16-bit attention. */
 FFWD_B200_API int ffwd_b200_precision(const ffwd_b200_ctx_t *ctx);
 
 /* Host-side LPT partition used by the sharder: assigns each of n items with
