@@ -1025,9 +1025,14 @@ int step_i8(ffwd_b200_ctx *ctx, Device &D, FwdState &fs, Workspace &w, int op, i
         p.err = w.err;
         return p;
     };
-    // LayerNorm of the residual stream (BERT), then its rows quantised; or the
-    // RMSNorm and quantisation in one.
+    // LayerNorm (BERT) or RMSNorm of the residual stream and its rows' codes, in
+    // one kernel but for wide LayerNorms.
     auto norm = [&](const float *g, const float *b) {
+        if (bert && i8_layernorm_quantize_fits(H)) {
+            LAUNCH(i8_layernorm_quantize_launch(w.x, g, b, eps, w.q8, w.q8_scale, T, H, D.num_sms,
+                                                s));
+            return 0;
+        }
         if (bert) {
             const RowOut xb{w.xb, nullptr, ctx->f16 ? 1 : 0, nullptr};
             LAUNCH(layernorm_launch(w.x, T, H, g, b, eps, xb, s));

@@ -61,6 +61,14 @@ int i8_quantize_launch(const void *x, int type, long long ldx, const float *norm
                        int8_t *q, long long ldq, float *s, int M, int K, int num_sms,
                        cudaStream_t stream);
 
+// LayerNorm of x [M, K] f32 in place (row stride K) with the rows' codes and
+// scales beside it; for the widths that fit (at most 1024, multiples of 16).
+// A row that is not finite, or below 1e-30 throughout, gets zeros.
+bool i8_layernorm_quantize_fits(int K);
+int i8_layernorm_quantize_launch(float *x, const float *gamma, const float *beta, float eps,
+                                 int8_t *q, float *s, int M, int K, int num_sms,
+                                 cudaStream_t stream);
+
 // Whether the streaming kernel for few rows (int8_vec.cu) takes this product.
 bool i8_vec_fits(int epi, const I8Params &p);
 int i8_vec_launch(int epi, const I8Params &p, int num_sms, cudaStream_t stream);

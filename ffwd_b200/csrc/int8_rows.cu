@@ -27,25 +27,29 @@ __device__ __forceinline__ float load1(const void *x, size_t i) {
     return __half2float(__ushort_as_half(h));
 }
 
+// How a row's columns map to loads: by element (kScalar: any K and alignment);
+// by four values (kFour: K and the addresses are multiples of four; columns
+// past K repeat the row's first ones, which changes no maximum); or by four
+// with every column inside (kFull: no bounds at all).
+enum Cover { kScalar, kFour, kFull };
+
 // Eight values of a row as loaded, columns [c, c + 4) and [c + 128, c + 132):
 // a warp whose lanes are 4 columns apart reads 256 columns in whole lines, of
 // the row and of f32 norm weights alike.  16-bit types stay packed: half the
 // registers, so twice the rows in flight.
-template <int TYPE, bool VEC>
+template <int TYPE, int COVER>
 struct Raw {
     uint32_t w[TYPE == kI8F32 ? 8 : 4];
 
-    // Columns at or past K read as 0.  VEC: K and the addresses are multiples of
-    // four values.
     __device__ __forceinline__ void load(const void *x, size_t off, int c, int K) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int ch = c + 128 * h;
+            int ch = c + 128 * h;
+            if (COVER == kFour) ch = ch < K ? ch : 0;
             if (TYPE == kI8F32) {
                 const uint32_t *p = static_cast<const uint32_t *>(x) + off + ch;
-                if (VEC) {
-                    uint4 r = make_uint4(0, 0, 0, 0);
-                    if (ch < K) r = __ldg(reinterpret_cast<const uint4 *>(p));
+                if (COVER != kScalar) {
+                    const uint4 r = __ldg(reinterpret_cast<const uint4 *>(p));
                     w[4 * h] = r.x;
                     w[4 * h + 1] = r.y;
                     w[4 * h + 2] = r.z;
@@ -56,9 +60,8 @@ struct Raw {
                 }
             } else {
                 const uint16_t *p = static_cast<const uint16_t *>(x) + off + ch;
-                if (VEC) {
-                    uint2 r = make_uint2(0, 0);
-                    if (ch < K) r = __ldg(reinterpret_cast<const uint2 *>(p));
+                if (COVER != kScalar) {
+                    const uint2 r = __ldg(reinterpret_cast<const uint2 *>(p));
                     w[2 * h] = r.x;
                     w[2 * h + 1] = r.y;
                 } else {
@@ -90,9 +93,9 @@ struct Raw {
     }
 };
 
-template <bool VEC>
+template <int COVER>
 __device__ __forceinline__ void load_norm(const float *w, int c, int K, float (&g)[8]) {
-    Raw<kI8F32, VEC> r;
+    Raw<kI8F32, COVER> r;
     r.load(w, 0, c, K);
     r.unpack(g);
 }
@@ -104,10 +107,10 @@ __device__ __forceinline__ double quotient(double v, double s, double rs) {
     return fma(fma(-t, s, v), rs, t);
 }
 
-// max(m, |v|), NaN if either is.
-__device__ __forceinline__ float max_abs(float m, float v) {
+// max(m, |a|, |b|), NaN if one is.
+__device__ __forceinline__ float max_abs(float m, float a, float b) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(v)));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
     return r;
 }
 
@@ -131,7 +134,7 @@ __device__ __forceinline__ float pick8(const float (&v)[8], int j) {
 // Codes of eight values (x, or x * g with a norm) of a row whose largest
 // magnitude is amax + amax_lo, written at columns c and c + 128 on.  With SETTLE, values next to a border are settled; without, the result
 // says whether there are any.
-template <bool NORM, bool SETTLE, bool VEC>
+template <bool NORM, bool SETTLE, int COVER>
 __device__ __forceinline__ bool put8(float (&x)[8], const float (&g)[8], float inv, float amax,
                                      float amax_lo, int8_t *q, int c, int K) {
     // How far the f32 quotient may be off: 127 x 2^-24 for the reciprocal's
@@ -147,7 +150,7 @@ __device__ __forceinline__ bool put8(float (&x)[8], const float (&g)[8], float i
         if (NORM) t = mul_f32x2(t, make_float2(g[2 * i], g[2 * i + 1]));
         const float2 f = fma_f32x2(t, inv2, up);
         const float2 r = fma_f32x2(t, inv2, fma_f32x2(f, minus, up));
-        far = fmaxf(far, fmaxf(fabsf(r.x), fabsf(r.y)));
+        far = max_abs(far, r.x, r.y);
         code[2 * i] = f.x;
         code[2 * i + 1] = f.y;
         d[2 * i] = r.x;
@@ -183,8 +186,8 @@ __device__ __forceinline__ bool put8(float (&x)[8], const float (&g)[8], float i
     for (int h = 0; h < 2; ++h) {
         const int ch = c + 128 * h;
         const uint32_t w = h ? w1 : w0;
-        if (VEC) {
-            if (ch < K) *reinterpret_cast<uint32_t *>(q + ch) = w;
+        if (COVER != kScalar) {
+            if (COVER == kFull || ch < K) *reinterpret_cast<uint32_t *>(q + ch) = w;
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -205,7 +208,7 @@ constexpr int min_blocks(int type, bool norm, int w, int nv) {
 // W warps per row, each thread holding NV groups of 8 columns (NV = 0: any
 // width, the row read again in each pass).  A block of max(W, 8) warps walks
 // over rows, the next row's loads in flight while it works on one.
-template <int TYPE, bool NORM, bool VEC, int W, int NV>
+template <int TYPE, bool NORM, int COVER, int W, int NV>
 __global__ void __launch_bounds__((W > 8 ? W : 8) * 32, min_blocks(TYPE, NORM, W, NV))
     quantize_kernel(const void *x, long long ldx, const float *norm, float eps, int8_t *q,
                     long long ldq, float *s, int M, int K) {
@@ -219,7 +222,7 @@ __global__ void __launch_bounds__((W > 8 ? W : 8) * 32, min_blocks(TYPE, NORM, W
     const int t = wr * 32 + lane;
     const int c0 = wr * 256 + lane * 4;  // first column of this thread's groups
     constexpr int NR = NV > 0 ? NV : 1;
-    Raw<TYPE, VEC> next[NR];
+    Raw<TYPE, COVER> next[NR];
     auto prefetch = [&](int row) {
         if (NV > 0 && row < M) {
 #pragma unroll
@@ -235,7 +238,7 @@ __global__ void __launch_bounds__((W > 8 ? W : 8) * 32, min_blocks(TYPE, NORM, W
         const int row = row0 + warp / W;
         const bool live = row < M;
         const size_t off = live ? (size_t)row * ldx : 0;
-        Raw<TYPE, VEC> raw[NR];
+        Raw<TYPE, COVER> raw[NR];
 #pragma unroll
         for (int k = 0; k < NR; ++k) raw[k] = next[k];
         if (M - row0 > stride) prefetch(row + stride);
@@ -247,33 +250,35 @@ __global__ void __launch_bounds__((W > 8 ? W : 8) * 32, min_blocks(TYPE, NORM, W
                 for (int k = 0; k < NR; ++k) {
                     const int c = k * W * 256 + c0;
                     raw[k].unpack(v);
-                    if (NORM) load_norm<VEC>(norm, c, K, g);
+                    if (NORM) load_norm<COVER>(norm, c, K, g);
                     f(v, g, c);
                 }
             } else {
                 for (int c = c0; c < K; c += W * 256) {
                     raw[0].load(x, off, c, K);
                     raw[0].unpack(v);
-                    if (NORM) load_norm<VEC>(norm, c, K, g);
+                    if (NORM) load_norm<COVER>(norm, c, K, g);
                     f(v, g, c);
                 }
             }
         };
         float2 m2 = make_float2(0.0f, 0.0f), s2 = m2;
         if (live)
-            each([&](const float(&a)[8], const float(&b)[8], int) {
+            each([&](const float(&a)[8], const float(&b)[8], int c) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float2 v = make_float2(a[2 * i], a[2 * i + 1]);
                     if (NORM) {
-                        s2 = fma_f32x2(v, v, s2);
+                        if (COVER != kFour || c + i / 2 * 128 < K) s2 = fma_f32x2(v, v, s2);
                         v = mul_f32x2(v, make_float2(b[2 * i], b[2 * i + 1]));
                     }
-                    m2.x = max_abs(m2.x, v.x);
-                    m2.y = max_abs(m2.y, v.y);
+                    if (i & 1)
+                        m2.x = max_abs(m2.x, v.x, v.y);
+                    else
+                        m2.y = max_abs(m2.y, v.x, v.y);
                 }
             });
-        const float mv = max_abs(m2.x, m2.y);
+        const float mv = max_abs(0.0f, m2.x, m2.y);
         float ss = s2.x + s2.y;
         // Magnitudes compare as unsigned integers, NaN above infinity.
         const uint32_t mine = __float_as_uint(mv);
@@ -310,7 +315,7 @@ __global__ void __launch_bounds__((W > 8 ? W : 8) * 32, min_blocks(TYPE, NORM, W
         bool open = false;  // codes left to settle
         if (plain)
             each([&](float(&a)[8], const float(&b)[8], int c) {
-                if (c < K) open |= put8<NORM, !NORM, VEC>(a, b, inv, amax, 0.0f, qr, c, K);
+                if (COVER == kFull || c < K) open |= put8<NORM, !NORM, COVER>(a, b, inv, amax, 0.0f, qr, c, K);
             });
         if (live && !plain) {
             // 127 / amax may pass f32 for rows so small: a value at a time, in
@@ -351,8 +356,96 @@ __global__ void __launch_bounds__((W > 8 ? W : 8) * 32, min_blocks(TYPE, NORM, W
             }
             if (open)
                 each([&](float(&a)[8], const float(&b)[8], int c) {
-                    if (c < K) put8<NORM, true, VEC>(a, b, inv, amax, lo, qr, c, K);
+                    if (COVER == kFull || c < K) put8<NORM, true, COVER>(a, b, inv, amax, lo, qr, c, K);
                 });
+        }
+    }
+}
+
+// LayerNorm of f32 rows in place, their codes written beside them: a warp per
+// row (at most NV x 256 columns), the row in registers, the next one's loads in
+// flight.  Replaces a LayerNorm and a quantisation (15 bytes a value with the
+// 16-bit copy between them) by 9 bytes a value.
+template <int COVER, int NV>
+__global__ void __launch_bounds__(256, 2)
+    layernorm_quantize_kernel(float *x, const float *gamma, const float *beta, float eps,
+                              int8_t *q, float *s, int M, int K) {
+    griddep_wait();
+    griddep_launch();
+    const int lane = threadIdx.x & 31;
+    const int stride = gridDim.x * 8;
+    int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    Raw<kI8F32, COVER> next[NV];
+    auto prefetch = [&](int r) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) next[k].load(x, (size_t)r * K, k * 256 + lane * 4, K);
+    };
+    auto sum = [&](float v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    };
+    if (row < M) prefetch(row);
+#pragma unroll 1
+    for (; row < M; row += stride) {
+        float v[NV][8];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) next[k].unpack(v[k]);
+        if (M - row > stride) prefetch(row + stride);
+        // (k, i) -> whether the value's column is inside the row
+        auto in = [&](int k, int i) {
+            return COVER == kFull || k * 256 + lane * 4 + i / 4 * 128 < K;
+        };
+        float acc = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (in(k, i)) acc += v[k][i];
+        const float mean = sum(acc) / (float)K;
+        acc = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[k][i] -= mean;
+                if (in(k, i)) acc = fmaf(v[k][i], v[k][i], acc);
+            }
+        const float inv_std = 1.0f / sqrtf(sum(acc) / (float)K + eps);
+        float mv = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = k * 256 + lane * 4;
+            float g[8], b[8];
+            load_norm<COVER>(gamma, c, K, g);
+            load_norm<COVER>(beta, c, K, b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[k][i] = fmaf(g[i] * v[k][i], inv_std, b[i]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (in(k, 4 * h))
+                    *reinterpret_cast<float4 *>(x + (size_t)row * K + c + 128 * h) = make_float4(
+                        v[k][4 * h], v[k][4 * h + 1], v[k][4 * h + 2], v[k][4 * h + 3]);
+            // (columns past the row repeat valid ones, through other weights' places)
+#pragma unroll
+            for (int i = 0; i < 8; i += 2)
+                if (in(k, i)) mv = max_abs(mv, v[k][i], v[k][i + 1]);
+        }
+        const uint32_t mx = __reduce_max_sync(0xffffffffu, __float_as_uint(mv));
+        const float amax = __uint_as_float(mx);
+        const bool finite = mx < 0x7F800000u;
+        if (lane == 0) s[row] = finite ? amax / 127.0f : __uint_as_float(0x7FC00000u);
+        const float inv = finite && amax >= 1e-30f ? 127.0f / amax : 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = k * 256 + lane * 4;
+            if (inv == 0.0f) {  // zeros, or not finite: no codes
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[k][i] = 0.0f;
+            }
+            if (COVER == kFull || c < K)
+                put8<false, true, COVER>(v[k], v[k], inv, inv == 0.0f ? 1.0f : amax, 0.0f,
+                                         q + (size_t)row * K, c, K);
         }
     }
 }
@@ -368,39 +461,53 @@ struct Args {
     int M, K, num_sms;
 };
 
-template <int TYPE, bool NORM, bool VEC, int W, int NV>
+template <int TYPE, bool NORM, int COVER, int W, int NV>
 cudaError_t run(const Args &a, cudaStream_t st) {
     constexpr int NW = W > 8 ? W : 8, R = NW / W;
     const int grid = std::min((a.M + R - 1) / R, a.num_sms * min_blocks(TYPE, NORM, W, NV));
-    return launch_k(quantize_kernel<TYPE, NORM, VEC, W, NV>, dim3(grid), dim3(NW * 32), 0, st, a.x,
-                    a.ldx, a.norm, a.eps, a.q, a.ldq, a.s, a.M, a.K);
+    return launch_k(quantize_kernel<TYPE, NORM, COVER, W, NV>, dim3(grid), dim3(NW * 32), 0, st,
+                    a.x, a.ldx, a.norm, a.eps, a.q, a.ldq, a.s, a.M, a.K);
+}
+
+// W warps a row, NV groups a thread where they cover the row exactly.
+template <int TYPE, bool NORM, int W>
+cudaError_t full(const Args &a, cudaStream_t st) {
+    switch (a.K / (W * 256)) {
+    case 1: return run<TYPE, NORM, kFull, W, 1>(a, st);
+    case 2: return run<TYPE, NORM, kFull, W, 2>(a, st);
+    case 3: return run<TYPE, NORM, kFull, W, 3>(a, st);
+    }
+    return run<TYPE, NORM, kFull, W, 4>(a, st);
 }
 
 // Many rows: as few warps per row as hold it (a warp's own reductions, no
-// block barrier).  Few rows (under two per SM): more warps per row, so that a
-// row's loads are all in flight at once.  Columns or addresses that are no
-// multiple of four values: by element, the row read again in each pass.
+// block barrier), without bounds where its width is a whole number of groups
+// (32768 x 1024 f32 with norm: 34 us with them).  Few rows (under two per SM):
+// more warps per row, so that a row's loads are all in flight at once.
+// Columns or addresses that are no multiple of four values: by element, the row
+// read again in each pass.
 template <int TYPE, bool NORM>
 cudaError_t pick(const Args &a, bool vec, cudaStream_t st) {
     const bool few = a.M < 2 * a.num_sms;
     if (!vec) {
-        return a.K <= 1024 && !few ? run<TYPE, NORM, false, 1, 0>(a, st)
-                                   : run<TYPE, NORM, false, 16, 0>(a, st);
+        return a.K <= 1024 && !few ? run<TYPE, NORM, kScalar, 1, 0>(a, st)
+                                   : run<TYPE, NORM, kScalar, 16, 0>(a, st);
     }
-    if (a.K <= 256) return run<TYPE, NORM, true, 1, 1>(a, st);
-    if (!few) {
-        if (a.K <= 512) return run<TYPE, NORM, true, 1, 2>(a, st);
-        if (a.K <= 1024) return run<TYPE, NORM, true, 1, 4>(a, st);
+    if (few) {
+        if (a.K <= 1024) return run<TYPE, NORM, kFour, 4, 1>(a, st);
+        if (a.K <= 4096) return run<TYPE, NORM, kFour, 16, 1>(a, st);
+    } else {
+        if (a.K <= 1024)
+            return a.K % 256 == 0   ? full<TYPE, NORM, 1>(a, st)
+                   : a.K <= 512 ? run<TYPE, NORM, kFour, 1, 2>(a, st)
+                                : run<TYPE, NORM, kFour, 1, 4>(a, st);
+        if (a.K <= 4096)
+            return a.K % 1024 == 0 ? full<TYPE, NORM, 4>(a, st)
+                                   : run<TYPE, NORM, kFour, 4, 4>(a, st);
+        if (a.K <= 16384 && a.K % 4096 == 0) return full<TYPE, NORM, 16>(a, st);
     }
-    if (a.K <= 1024) return run<TYPE, NORM, true, 4, 1>(a, st);
-    if (!few) {
-        if (a.K <= 2048) return run<TYPE, NORM, true, 4, 2>(a, st);
-        if (a.K <= 4096) return run<TYPE, NORM, true, 4, 4>(a, st);
-    }
-    if (a.K <= 4096) return run<TYPE, NORM, true, 16, 1>(a, st);
-    if (a.K <= 8192) return run<TYPE, NORM, true, 16, 2>(a, st);
-    if (a.K <= 16384) return run<TYPE, NORM, true, 16, 4>(a, st);
-    return run<TYPE, NORM, true, 16, 0>(a, st);
+    if (a.K <= 16384) return run<TYPE, NORM, kFour, 16, 4>(a, st);
+    return run<TYPE, NORM, kFour, 16, 0>(a, st);
 }
 
 }  // namespace
@@ -419,6 +526,24 @@ int i8_quantize_launch(const void *x, int type, long long ldx, const float *norm
     case kI8F16: return norm ? pick<kI8F16, true>(a, vec, stream) : pick<kI8F16, false>(a, vec, stream);
     }
     return cudaErrorInvalidValue;
+}
+
+bool i8_layernorm_quantize_fits(int K) { return K <= 1024 && K % 16 == 0; }
+
+int i8_layernorm_quantize_launch(float *x, const float *gamma, const float *beta, float eps,
+                                 int8_t *q, float *s, int M, int K, int num_sms,
+                                 cudaStream_t stream) {
+    const int grid = std::min((M + 7) / 8, num_sms * 2);
+    auto go = [&](auto kern) {
+        return launch_k(kern, dim3(grid), dim3(256), 0, stream, x, gamma, beta, eps, q, s, M, K);
+    };
+    switch (K) {
+    case 256: return go(layernorm_quantize_kernel<kFull, 1>);
+    case 512: return go(layernorm_quantize_kernel<kFull, 2>);
+    case 768: return go(layernorm_quantize_kernel<kFull, 3>);
+    case 1024: return go(layernorm_quantize_kernel<kFull, 4>);
+    }
+    return K <= 512 ? go(layernorm_quantize_kernel<kFour, 2>) : go(layernorm_quantize_kernel<kFour, 4>);
 }
 
 }  // namespace fb
