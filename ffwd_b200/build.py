@@ -28,7 +28,7 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVFLAGS = ARCH + ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-fvisibility=hidden",
                   "--expt-relaxed-constexpr", "-I" + os.path.join(ROOT, "include")]
 CU_SRCS = ["gemm.cu", "gemm2.cu", "attention.cu", "rowops.cu", "late.cu",
-           "int8_rows.cu", "int8_gemm.cu", "int8_vec.cu", "int8_api.cu", "engine.cu"]
+           "int8_rows.cu", "int8_gemm.cu", "int8_mid.cu", "int8_vec.cu", "int8_api.cu", "engine.cu"]
 CC_SRCS = ["loader.cc"]
 
 LIB = os.path.join(LIBDIR, "libffwd_b200.so")

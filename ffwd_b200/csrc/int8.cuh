@@ -73,6 +73,10 @@ int i8_layernorm_quantize_launch(float *x, const float *gamma, const float *beta
 bool i8_vec_fits(int epi, const I8Params &p);
 int i8_vec_launch(int epi, const I8Params &p, int num_sms, cudaStream_t stream);
 
+// Kernel for a few tens of rows (int8_mid.cu): likewise; -1 with a message, or 0.
+bool i8_mid_fits(int epi, const I8Params &p, int num_sms);
+int i8_mid_run(int epi, const I8Params &p, int num_sms, cudaStream_t stream);
+
 // Tensor-core kernel (int8_gemm.cu).  -1 with a message, or 0.
 int i8_gemm_run(int epi, const I8Params &p, int num_sms, cudaStream_t stream);
 

@@ -30,11 +30,14 @@ int device_info(int *dev, int *sms) {
     return 0;
 }
 
+// Rows of one call: tile arithmetic stays within 32 bits.
+constexpr int kMaxRows = 1 << 30;
+
 bool type_ok(int t) { return t == kI8F32 || t == kI8BF16 || t == kI8F16; }
 
 // Shapes, strides and alignment of the quantised rows.
 int check_rows(const int8_t *x, long long ldx, const float *xs, int M, int K) {
-    if (M < 0 || !x || !xs) {
+    if (M < 0 || M > kMaxRows || !x || !xs) {
         fail("invalid arguments");
         return -1;
     }
@@ -52,7 +55,7 @@ int check_rows(const int8_t *x, long long ldx, const float *xs, int M, int K) {
 }
 
 int check_mat(const ffwd_b200_i8_mat_t *w) {
-    if (!w || !w->q || !w->scale || w->rows <= 0 || w->cols <= 0) {
+    if (!w || !w->q || !w->scale || w->rows <= 0 || w->rows > kMaxRows || w->cols <= 0) {
         fail("invalid weights");
         return -1;
     }
@@ -118,6 +121,7 @@ int i8_project(int epi, const I8Params &p, int num_sms, cudaStream_t stream) {
         LAUNCH(i8_vec_launch(epi, p, num_sms, stream));
         return 0;
     }
+    if (i8_mid_fits(epi, p, num_sms)) return i8_mid_run(epi, p, num_sms, stream);
     return i8_gemm_run(epi, p, num_sms, stream);
 }
 
@@ -131,7 +135,8 @@ FFWD_B200_API int ffwd_b200_quantize_i8(const void *x, int type, long long ldx, 
                                         float eps, int8_t *q, long long ldq, float *scale, int M,
                                         int K, void *stream) {
     clear_error();
-    if (!x || !q || !scale || !type_ok(type) || M < 0 || K <= 0) {
+    if (!x || !q || !scale || !type_ok(type) || M < 0 || M > kMaxRows || K <= 0 ||
+        K > kMaxRows) {
         fail("invalid arguments");
         return -1;
     }

@@ -51,14 +51,16 @@ __device__ __forceinline__ float2 over_1p(float2 x, float2 d) {
 // SiLU, x / (1 + 2^e), e = -x log2(e): e in two parts (its rounding alone would
 // be off by |x| 2^-24 of the result for negative x).
 __device__ __forceinline__ float2 silu(float2 x) {
-    const float2 e = mul_f32x2(x, both(-1.44269504f));
+    // (beyond 200 the result is x or 0, and the parts would pass f32)
+    const float2 c = make_float2(fminf(fmaxf(x.x, -200.0f), 200.0f),
+                                 fminf(fmaxf(x.y, -200.0f), 200.0f));
+    const float2 e = mul_f32x2(c, both(-1.44269504f));
     const float2 ne = make_float2(-e.x, -e.y);
-    const float2 lo = fma_f32x2(x, both(-1.92596299e-8f), fma_f32x2(x, both(-1.44269504f), ne));
+    const float2 lo = fma_f32x2(c, both(-1.92596299e-8f), fma_f32x2(c, both(-1.44269504f), ne));
     const float2 w = make_float2(ex2_approx(e.x), ex2_approx(e.y));
-    // (an infinite power times a zero or infinite lo would be NaN)
-    const float2 cor = mul_f32x2(lo, both(0.69314718f));
+    // (an infinite power times a lo of zero would be NaN)
     const float2 wf = make_float2(fminf(w.x, 3.0e38f), fminf(w.y, 3.0e38f));
-    return over_1p(x, fma_f32x2(wf, cor, w));
+    return over_1p(x, fma_f32x2(wf, mul_f32x2(lo, both(0.69314718f)), w));
 }
 
 // GELU, tanh form: 0.5 (1 + tanh(v)) = 1 / (1 + 2^e), v = sqrt(2 / pi) (x +

@@ -1,0 +1,425 @@
+// 8-bit integer projections of a few tens of rows (see int8.cuh): latency and
+// the weights' bytes bound them, not the products.  The operands change
+// places, tcgen05.mma kind::i8 with 128 weight rows as M and T <= 128 quantised
+// rows as N, so a weight byte costs T / 256 of the tensor work that the 256-row
+// tiles of int8_gemm.cu spend on it; and where there are fewer 128-channel
+// tiles than SMs, a cluster of S CTAs splits K: their integer sums meet in
+// distributed shared memory, each CTA finishing T / S of the rows (exact, so
+// the split changes no bit).  An accumulator column is a row of the result: a
+// thread holds one channel (its scale and bias in registers), a warp stores 32
+// neighbouring channels.
+//
+// One tile per CTA.  Warp 0 TMA producer, warp 1 TMEM allocation and MMA issue,
+// warps 2-9 the epilogue: two warpgroups that take turns at 8 rows.
+#include "host_util.h"
+#include "int8.cuh"
+#include "int8_epi.cuh"
+#include "launch_util.cuh"
+#include "ptx.cuh"
+
+#include <algorithm>
+
+namespace fb {
+namespace {
+
+constexpr int BK = 128;   // bytes of K per stage
+constexpr int BC = 128;   // channels per tile
+constexpr int kThreads = 64 + 256;
+constexpr int kRows = 8;  // rows an epilogue warpgroup works on at once
+
+template <int EPI, int T>
+struct Cfg {
+    static constexpr int MATS = EPI == kI8Gated ? 2 : 1;
+    static constexpr int W_BYTES = BC * BK;
+    static constexpr int STAGE = MATS * W_BYTES + T * BK;
+    static constexpr int STAGES = 196608 / STAGE > 8 ? 8 : 196608 / STAGE;
+    static constexpr int SMEM = STAGES * STAGE + 1024;
+    static constexpr int TMEM_COLS = MATS * T < 32 ? 32 : MATS * T;
+    // After the products the stages hold the sums [MATS][T][BC] and, in the head
+    // form, values [T][BC] and partial sums of squares [T][4].
+    static constexpr int OFF_VALUES = MATS * T * BC * 4;
+    static_assert(OFF_VALUES + (EPI == kI8Heads ? T * (BC + 4) * 4 : 0) <= STAGES * STAGE,
+                  "the sums fit the stages");
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                     : "memory");
+}
+
+// The int at this shared-memory address in CTA `rank` of the cluster.
+__device__ __forceinline__ int load_peer(uint32_t addr, uint32_t rank) {
+    int v;
+    asm volatile(
+        "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\t"
+        "ld.shared::cluster.s32 %0, [a];\n\t}"
+        : "=r"(v)
+        : "r"(addr), "r"(rank)
+        : "memory");
+    return v;
+}
+
+__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                        uint32_t idesc, uint32_t accum) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accum)
+        : "memory");
+}
+
+// kind::i8: s32 accumulate, both operands signed, K-major.
+constexpr uint32_t idesc_i8(int M, int N) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) |
+           ((uint32_t)(M >> 4) << 24);
+}
+
+template <int EPI, int T, int HD>
+__global__ void __launch_bounds__(kThreads)
+    i8_mid_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmW2,
+                  const __grid_constant__ CUtensorMap tmX, const I8Params p, const int split) {
+    extern __shared__ uint8_t smem_raw[];
+    using CF = Cfg<EPI, T>;
+    constexpr int STAGES = CF::STAGES;
+    __shared__ __align__(8) uint64_t full_bar[STAGES];
+    __shared__ __align__(8) uint64_t empty_bar[STAGES];
+    __shared__ __align__(8) uint64_t done_bar;
+    __shared__ uint32_t tmem_base_sh;
+    __shared__ int abort_sh;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint8_t *smem = reinterpret_cast<uint8_t *>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    const int rank = split > 1 ? (int)cluster_rank() : 0;
+    const int c0 = blockIdx.x / split * BC;  // first channel
+    const int row0 = blockIdx.y * T;         // first row
+    const int k_blocks = (p.K + BK - 1) / BK;
+    const int kb0 = k_blocks * rank / split, kb1 = k_blocks * (rank + 1) / split;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&empty_bar[s], 1);
+        }
+        mbar_init(&done_bar, 1);
+        abort_sh = 0;
+        fence_barrier_init();
+        tma_prefetch_desc(&tmW);
+        if (EPI == kI8Gated) tma_prefetch_desc(&tmW2);
+        tma_prefetch_desc(&tmX);
+    }
+    if (warp == 1) {
+        tmem_alloc(&tmem_base_sh, CF::TMEM_COLS);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base_sh;
+    // The first weights on their way to L2 while the stream's previous kernel
+    // (as a rule the one that quantises the rows) still runs.
+    if (threadIdx.x == 0) {
+        for (int kb = kb0; kb < kb1 && kb < kb0 + STAGES; ++kb) {
+            tma_prefetch_l2(&tmW, kb * BK, c0);
+            if (EPI == kI8Gated) tma_prefetch_l2(&tmW2, kb * BK, c0);
+        }
+    }
+    griddep_wait();
+    griddep_launch();
+
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int s = it % STAGES;
+                if (!mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1, p.err, &abort_sh)) {
+                    ok = false;
+                    break;
+                }
+                uint8_t *st = smem + s * CF::STAGE;
+                mbar_arrive_expect_tx(&full_bar[s], CF::STAGE);
+                tma_load_2d(st, &tmW, &full_bar[s], kb * BK, c0);
+                if (EPI == kI8Gated)
+                    tma_load_2d(st + CF::W_BYTES, &tmW2, &full_bar[s], kb * BK, c0);
+                tma_load_2d(st + CF::MATS * CF::W_BYTES, &tmX, &full_bar[s], kb * BK, row0);
+            }
+            // Its copies have landed before the stages are used for anything else.
+            for (int j = std::max(0, it - STAGES); j < it; ++j)
+                if (!mbar_wait(&full_bar[j % STAGES], (j / STAGES) & 1, p.err, nullptr)) ok = false;
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t IDESC = idesc_i8(BC, T);
+            int it = 0;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int s = it % STAGES;
+                if (!mbar_wait(&full_bar[s], (it / STAGES) & 1, p.err, &abort_sh)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t sw = smem_u32(smem + s * CF::STAGE);
+                const uint32_t sx = sw + CF::MATS * CF::W_BYTES;
+#pragma unroll
+                for (int kk = 0; kk < BK / 32; ++kk) {
+                    const uint64_t xd = smem_desc(sx + kk * 32, 16, 1024, kLayoutSW128);
+#pragma unroll
+                    for (int m = 0; m < CF::MATS; ++m)
+                        umma_i8(tmem + m * T,
+                                smem_desc(sw + m * CF::W_BYTES + kk * 32, 16, 1024, kLayoutSW128),
+                                xd, IDESC, (it | kk) != 0);
+                }
+                umma_commit(&empty_bar[s]);
+            }
+            umma_commit(&done_bar);
+            if (!mbar_wait(&done_bar, 0, p.err, nullptr)) ok = false;
+        }
+        __syncwarp();
+    }
+    // Every thread learns whether the products are complete (this also holds the
+    // epilogue back until they are).
+    ok = __syncthreads_and(ok);
+    tc_fence_after();
+    int *sums = reinterpret_cast<int *>(smem);  // [MATS][T][BC]
+    const int n = (warp & 3) * 32 + lane;       // channel of the tile (epilogue warps)
+    const int g = (warp - 2) >> 2;              // warpgroup
+    if (warp >= 2 && ok) {
+        const uint32_t tbase = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+#pragma unroll 1
+        for (int c = g * 16; c < CF::MATS * T; c += 32) {
+            float v[16];
+            tmem_ld16(tbase + c, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sums[(c + i) * BC + n] = __float_as_int(v[i]);
+        }
+        tc_fence_before();
+    }
+    if (split > 1) cluster_sync();
+    else __syncthreads();
+    if (warp >= 2 && ok) {
+        const int per = T / split, t0 = rank * per;
+        const int col = c0 + n;
+        const bool in = col < p.N;
+        const float ws = in ? __ldg(p.ws + col) : 0.0f;
+        const float b = in && p.bias ? __ldg(p.bias + col) : 0.0f;
+        float ws2 = 0.0f, b2 = 0.0f;
+        if (EPI == kI8Gated && in) {
+            ws2 = __ldg(p.ws2 + col);
+            if (p.bias2) b2 = __ldg(p.bias2 + col);
+        }
+        // Rows [t, t + kRows) of the sums m, over the cluster: all loads of a CTA's
+        // sums in flight at once.
+        auto total = [&](int m, int t, int(&a)[kRows]) {
+            const uint32_t at = smem_u32(sums + (m * T + t) * BC + n);
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) a[i] = 0;
+            if (split == 1) {
+#pragma unroll
+                for (int i = 0; i < kRows; ++i)
+                    if (t + i < T) a[i] = sums[(m * T + t + i) * BC + n];
+                return;
+            }
+#pragma unroll 2
+            for (int r = 0; r < split; ++r) {
+                int v[kRows];
+#pragma unroll
+                for (int i = 0; i < kRows; ++i) v[i] = t + i < t0 + per ? load_peer(at + i * BC * 4, r) : 0;
+#pragma unroll
+                for (int i = 0; i < kRows; ++i) a[i] += v[i];
+            }
+        };
+        const int t1 = min(t0 + per, p.M - row0);
+        // y = x w^T of rows [t, t + kRows), each as acc * s * w + b.
+        auto values8 = [&](int m, int t, float w, float bias, const float(&s)[kRows],
+                           float(&y)[kRows]) {
+            int a[kRows];
+            total(m, t, a);
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) y[i] = fmaf((float)a[i] * s[i], w, bias);
+        };
+        auto scales8 = [&](int t, float(&s)[kRows]) {
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) s[i] = t + i < t1 ? __ldg(p.xs + row0 + t + i) : 0.0f;
+        };
+        auto store8 = [&](int t, const float(&y)[kRows]) {
+            if (!in) return;
+#pragma unroll
+            for (int i = 0; i < kRows; ++i)
+                if (t + i < t1)
+                    i8::store1(p.y, p.type, (size_t)(row0 + t + i) * p.ldy + col, y[i],
+                                p.accumulate);
+        };
+        if constexpr (EPI != kI8Heads) {
+#pragma unroll 1
+            for (int t = t0 + g * kRows; t < t1; t += 2 * kRows) {
+                float s[kRows], y[kRows];
+                scales8(t, s);
+                values8(0, t, ws, b, s, y);
+                if (p.act != kI8None) {
+#pragma unroll
+                    for (int i = 0; i < kRows; i += 2) {
+                        const float2 v = i8::act2(make_float2(y[i], y[i + 1]), p.act);
+                        y[i] = v.x;
+                        y[i + 1] = v.y;
+                    }
+                }
+                if (EPI == kI8Gated) {
+                    float u[kRows];
+                    values8(1, t, ws2, b2, s, u);
+#pragma unroll
+                    for (int i = 0; i < kRows; ++i) y[i] *= u[i];
+                }
+                store8(t, y);
+            }
+        } else {
+            // A tile holds BC / HD whole heads; HD / 32 warps a head.
+            float *values = reinterpret_cast<float *>(smem + CF::OFF_VALUES);  // [T][BC]
+            float *part = values + T * BC;                                     // [T][4]
+            const int head = col / HD, e = n % HD, first = n / HD * (HD / 32);
+            const bool rot = head < p.n_q_heads + p.n_kv_heads;
+            const float *nw = !rot ? nullptr : head < p.n_q_heads ? p.q_norm : p.k_norm;
+            // The other value of this one's rotation, and its sign.
+            const int half = HD / 2, pair = e < half ? n + half : n - half;
+            const float sign = e < half ? -1.0f : 1.0f;
+            const float w1 = nw ? __ldg(nw + e) : 1.0f;
+            const float w2 = nw ? __ldg(nw + (e < half ? e + half : e - half)) : 1.0f;
+#pragma unroll 1
+            for (int t = t0 + g * kRows; t < t1; t += 2 * kRows) {
+                float s[kRows], y[kRows], cs[kRows], sn[kRows];
+                scales8(t, s);
+                uint32_t bad = 0;
+#pragma unroll
+                for (int i = 0; i < kRows; ++i) {
+                    const int ps = rot && t + i < t1 ? __ldg(p.pos + row0 + t + i) : 0;
+                    const bool out = ps < 0 || ps >= p.n_pos;
+                    bad |= (uint32_t)out << i;
+                    const size_t at = (size_t)(out ? 0 : ps) * half + e % half;
+                    cs[i] = __ldg(p.cos + at);
+                    sn[i] = __ldg(p.sin + at);
+                }
+                if (bad && in) set_error(p.err, kErrBadPosition);
+                values8(0, t, ws, b, s, y);
+                if (rot || HD == 64) {  // (a tile of two heads: all of its warps meet)
+                    float ss[kRows];
+#pragma unroll
+                    for (int i = 0; i < kRows; ++i) {
+                        ss[i] = y[i] * y[i];
+                        values[(t + i) % T * BC + n] = y[i];
+                    }
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                        for (int i = 0; i < kRows; ++i)
+                            ss[i] += __shfl_xor_sync(0xffffffffu, ss[i], o);
+                    if (lane == 0) {
+#pragma unroll
+                        for (int i = 0; i < kRows; ++i) part[(t + i) % T * 4 + (warp & 3)] = ss[i];
+                    }
+                    named_bar(1 + g, 128);
+                }
+                if (rot) {
+#pragma unroll
+                    for (int i = 0; i < kRows; ++i) {
+                        const int tt = (t + i) % T;
+                        float inv = bad >> i & 1 ? i8::nan_f() : 1.0f;
+                        if (nw) {
+                            float ss = 0.0f;
+#pragma unroll
+                            for (int k = 0; k < HD / 32; ++k) ss += part[tt * 4 + first + k];
+                            inv *= 1.0f / sqrtf(ss / (float)HD + p.eps);
+                        }
+                        y[i] = y[i] * inv * w1 * cs[i] +
+                               sign * (values[tt * BC + pair] * inv * w2 * sn[i]);
+                    }
+                }
+                store8(t, y);
+            }
+        }
+    }
+    if (split > 1) cluster_sync();  // no CTA leaves while its sums are read
+    else __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, CF::TMEM_COLS);
+    }
+}
+
+template <int EPI, int T, int HD>
+int launch(const I8Params &p, int split, cudaStream_t stream) {
+    CUtensorMap mw, mw2, mx;
+    constexpr CUtensorMapDataType U8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    constexpr CUtensorMapSwizzle SW = CU_TENSOR_MAP_SWIZZLE_128B;
+    if (make_map_ld(&mw, p.w, p.N, p.K, p.ldw, BC, BK, SW, U8, 1) ||
+        make_map_ld(&mx, p.x, p.M, p.K, p.ldx, T, BK, SW, U8, 1))
+        return -1;
+    mw2 = mw;
+    if (EPI == kI8Gated && make_map_ld(&mw2, p.w2, p.N, p.K, p.ldw2, BC, BK, SW, U8, 1)) return -1;
+    CK((set_smem_once<i8_mid_kernel<EPI, T, HD>>(Cfg<EPI, T>::SMEM)));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((p.N + BC - 1) / BC * split, (p.M + T - 1) / T);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Cfg<EPI, T>::SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = split;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    LAUNCH(cudaLaunchKernelEx(&cfg, i8_mid_kernel<EPI, T, HD>, mw, mw2, mx, p, split));
+    return 0;
+}
+
+template <int EPI, int HD>
+int launch_t(const I8Params &p, int split, cudaStream_t stream) {
+    if (p.M <= 16) return launch<EPI, 16, HD>(p, split, stream);
+    if (p.M <= 32) return launch<EPI, 32, HD>(p, split, stream);
+    if constexpr (EPI != kI8Heads) {
+        if (p.M > 64) return launch<EPI, 128, HD>(p, split, stream);
+    }
+    return launch<EPI, 64, HD>(p, split, stream);
+}
+
+}  // namespace
+
+// Up to 64 rows.  More, where K is long: the 256-row tiles of int8_gemm.cu do
+// not split it (4096 channels, K = 12288: 128 rows 16.6 us here, 34.3 there; 256
+// rows 25.5 and 34.6; 1024 channels, K = 2048, 128 rows: 10.1 and 8.8; heads of
+// K = 4096, 128 rows: 23.5 and 17.2), unless they fill the SMs.
+bool i8_mid_fits(int epi, const I8Params &p, int num_sms) {
+    if (p.M <= 64) return true;
+    if (epi == kI8Heads) return false;
+    if (p.M <= 128) return p.K >= 4096;
+    const long long cols = epi == kI8Gated ? 2ll * p.N : p.N;
+    return p.M <= 256 && p.K >= 8192 && (cols + 255) / 256 * 4 <= num_sms;
+}
+
+int i8_mid_run(int epi, const I8Params &p, int num_sms, cudaStream_t stream) {
+    // Split K until the CTAs fill the SMs, as long as each keeps two stages' worth.
+    const long long tiles = (p.N + BC - 1ll) / BC * ((p.M + 127) / 128);
+    const int k_blocks = (p.K + BK - 1) / BK;
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= num_sms && k_blocks >= 4 * split) split *= 2;
+    switch (epi) {
+    case kI8Store: return launch_t<kI8Store, 0>(p, split, stream);
+    case kI8Gated: return launch_t<kI8Gated, 0>(p, split, stream);
+    case kI8Heads:
+        return p.head_dim == 128 ? launch_t<kI8Heads, 128>(p, split, stream)
+                                 : launch_t<kI8Heads, 64>(p, split, stream);
+    }
+    return -1;
+}
+
+}  // namespace fb

@@ -234,14 +234,14 @@ __global__ void __launch_bounds__((W > 8 ? W : 8) * 32, min_blocks(TYPE, NORM, W
     prefetch(blockIdx.x * R + warp / W);
     // (the block's rounds are counted by its first row: all of its warps take part)
 #pragma unroll 1
-    for (int row0 = blockIdx.x * R; row0 < M; row0 += stride) {
-        const int row = row0 + warp / W;
+    for (int left = M - blockIdx.x * R; left > 0; left -= stride) {
+        const int row = M - left + warp / W;
         const bool live = row < M;
         const size_t off = live ? (size_t)row * ldx : 0;
         Raw<TYPE, COVER> raw[NR];
 #pragma unroll
         for (int k = 0; k < NR; ++k) raw[k] = next[k];
-        if (M - row0 > stride) prefetch(row + stride);
+        if (left > stride) prefetch(row + stride);
         // Each of the passes over the row below: from registers, or loaded again.
         auto each = [&](auto f) {
             float v[8], g[8];

@@ -16,7 +16,6 @@
 namespace fb {
 namespace {
 
-constexpr int kMaxRows = 8;
 
 __device__ __forceinline__ uint4 ldg16(const int8_t *p) {
     return __ldg(reinterpret_cast<const uint4 *>(p));
@@ -106,18 +105,28 @@ __device__ __forceinline__ float scaled(int acc, float s, const float *ws, const
     return fmaf((float)acc * s, __ldg(ws + n), bias ? __ldg(bias + n) : 0.0f);
 }
 
+// The first 2 KB of a row on their way to L2; before the wait for the stream's
+// previous kernel (as a rule the one that quantises the rows).
+__device__ __forceinline__ void prefetch_row(const int8_t *w, int K, int lane) {
+    if (lane * 128 < min(K, 2048))
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(w + lane * 128));
+}
+
 constexpr int kWarps = 4;
 
 template <int R, int MT>
 __global__ void __launch_bounds__(kWarps * 32) vec_store_kernel(const I8Params p) {
-    griddep_wait();
-    griddep_launch();
     const int lane = threadIdx.x & 31;
     const int n0 = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * R;
-    if (n0 >= p.N) return;
     const int8_t *w[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) w[r] = p.w + (size_t)min(n0 + r, p.N - 1) * p.ldw;
+    for (int r = 0; r < R; ++r) {
+        w[r] = p.w + (size_t)min(n0 + r, p.N - 1) * p.ldw;
+        prefetch_row(w[r], p.K, lane);
+    }
+    griddep_wait();
+    griddep_launch();
+    if (n0 >= p.N) return;
     int acc[R][MT];
     dots<R, MT>(w, p, lane, acc);
     const int a = mine<R, MT>(acc, lane);
@@ -130,17 +139,19 @@ __global__ void __launch_bounds__(kWarps * 32) vec_store_kernel(const I8Params p
 // R columns of gate and up each.
 template <int R, int MT>
 __global__ void __launch_bounds__(kWarps * 32) vec_gated_kernel(const I8Params p) {
-    griddep_wait();
-    griddep_launch();
     const int lane = threadIdx.x & 31;
     const int n0 = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * R;
-    if (n0 >= p.N) return;
     const int8_t *w[2 * R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         w[r] = p.w + (size_t)min(n0 + r, p.N - 1) * p.ldw;
         w[R + r] = p.w2 + (size_t)min(n0 + r, p.N - 1) * p.ldw2;
+        prefetch_row(w[r], p.K, lane);
+        prefetch_row(w[R + r], p.K, lane);
     }
+    griddep_wait();
+    griddep_launch();
+    if (n0 >= p.N) return;
     int acc[2 * R][MT];
     dots<2 * R, MT>(w, p, lane, acc);
     const int v = mine<2 * R, MT>(acc, lane);
@@ -158,11 +169,14 @@ constexpr int kHeadWarps = 16;
 template <int HD, int MT>
 __global__ void __launch_bounds__(kHeadWarps * 32) vec_heads_kernel(const I8Params p) {
     __shared__ float v[MT][HD];
-    griddep_wait();
-    griddep_launch();
     constexpr int R = 4, HALF = HD / 2;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int head = blockIdx.x;
+    for (int e0 = warp * R; e0 < HD; e0 += kHeadWarps * R)
+        for (int r = 0; r < R; ++r)
+            prefetch_row(p.w + (size_t)(head * HD + e0 + r) * p.ldw, p.K, lane);
+    griddep_wait();
+    griddep_launch();
     for (int e0 = warp * R; e0 < HD; e0 += kHeadWarps * R) {
         const int n0 = head * HD + e0;
         const int8_t *w[R];
@@ -230,16 +244,17 @@ cudaError_t run_gated(const I8Params &p, cudaStream_t st) {
 }
 
 // More weight rows per warp once there are enough of them to fill the SMs'
-// warps: the rows' loads are shared among them.
+// warps, and with more quantised rows: a warp's loads of those are shared among
+// its weight rows.
 template <int MT>
 cudaError_t run(int epi, const I8Params &p, int num_sms, cudaStream_t st) {
     const int warps = num_sms * 16;
     switch (epi) {
     case kI8Store:
-        return p.N >= 4 * warps   ? run_store<4, MT>(p, st)
-               : p.N >= 2 * warps ? run_store<2, MT>(p, st)
-                                  : run_store<1, MT>(p, st);
-    case kI8Gated: return p.N >= 2 * warps ? run_gated<2, MT>(p, st) : run_gated<1, MT>(p, st);
+        if (MT == 4 || p.N >= 4 * warps) return run_store<4, MT>(p, st);
+        return MT == 2 || p.N >= 2 * warps ? run_store<2, MT>(p, st) : run_store<1, MT>(p, st);
+    case kI8Gated:
+        return MT == 4 || p.N >= 2 * warps ? run_gated<2, MT>(p, st) : run_gated<1, MT>(p, st);
     case kI8Heads: {
         const int heads = p.n_q_heads + 2 * p.n_kv_heads;
         return p.head_dim == 128 ? launch_k(vec_heads_kernel<128, MT>, dim3(heads),
@@ -253,13 +268,17 @@ cudaError_t run(int epi, const I8Params &p, int num_sms, cudaStream_t st) {
 
 }  // namespace
 
-bool i8_vec_fits(int, const I8Params &p) { return p.M <= kMaxRows; }
+// Up to 2 rows; 3 and 4 while the weights are under 16 MB (4096 x 12288 with 4
+// rows: 21 us against 12.5 of int8_mid.cu; 8192 x 1024: 4.0 against 5.9).
+bool i8_vec_fits(int epi, const I8Params &p) {
+    if (p.M <= 2) return true;
+    return p.M <= 4 && (long long)p.N * p.K * (epi == kI8Gated ? 2 : 1) <= 16 << 20;
+}
 
 int i8_vec_launch(int epi, const I8Params &p, int num_sms, cudaStream_t stream) {
     if (p.M <= 1) return run<1>(epi, p, num_sms, stream);
     if (p.M <= 2) return run<2>(epi, p, num_sms, stream);
-    if (p.M <= 4) return run<4>(epi, p, num_sms, stream);
-    return run<8>(epi, p, num_sms, stream);
+    return run<4>(epi, p, num_sms, stream);
 }
 
 }  // namespace fb

@@ -509,30 +509,31 @@ def _i8_check(rc, what):
 def quantize_i8(x_ptr, dtype, ldx, q_ptr, ldq, scale_ptr, M, K, norm_ptr=None, eps=0.0, stream=0):
     """Rows to int8 with a scale each, optionally after an RMSNorm with weights
     at norm_ptr."""
-    _i8_check(lib().ffwd_b200_quantize_i8(x_ptr, _i8_code(I8_TYPES, dtype), ldx, norm_ptr, eps, q_ptr, ldq,
-                                          scale_ptr, M, K, stream), "quantize_i8")
+    _i8_check(lib().ffwd_b200_quantize_i8(x_ptr, _i8_code(I8_TYPES, dtype), ldx, norm_ptr, eps,
+                                          q_ptr, ldq, scale_ptr, M, K, stream), "quantize_i8")
 
 
 def gemm_i8(w, x_ptr, ldx, xs_ptr, M, y_ptr, dtype, ldy, act="none", accumulate=False,
             err_ptr=None, stream=0):
     """y = act(x w^T) (accumulate: y +=) of quantised rows with weights `w` (i8_mat)."""
     _i8_check(lib().ffwd_b200_gemm_i8(ctypes.byref(w), x_ptr, ldx, xs_ptr, M, y_ptr,
-                                      _i8_code(I8_TYPES, dtype), ldy, _i8_code(I8_ACTS, act), int(accumulate),
-                                      err_ptr, stream), "gemm_i8")
+                                      _i8_code(I8_TYPES, dtype), ldy, _i8_code(I8_ACTS, act),
+                                      int(accumulate), err_ptr, stream), "gemm_i8")
 
 
 def gated_i8(gate, up, x_ptr, ldx, xs_ptr, M, h_ptr, dtype, ldh, act="silu", err_ptr=None,
              stream=0):
     """h = act(x gate^T) * (x up^T) of quantised rows."""
     _i8_check(lib().ffwd_b200_gated_i8(ctypes.byref(gate), ctypes.byref(up), x_ptr, ldx, xs_ptr, M,
-                                       h_ptr, _i8_code(I8_TYPES, dtype), ldh, _i8_code(I8_ACTS, act), err_ptr,
-                                       stream), "gated_i8")
+                                       h_ptr, _i8_code(I8_TYPES, dtype), ldh,
+                                       _i8_code(I8_ACTS, act), err_ptr, stream), "gated_i8")
 
 
 def qkv_i8(w, heads, x_ptr, ldx, xs_ptr, M, out_ptr, dtype, ldo, err_ptr=None, stream=0):
     """Fused QKV projection of quantised rows, head norms and rotation included."""
     _i8_check(lib().ffwd_b200_qkv_i8(ctypes.byref(w), ctypes.byref(heads), x_ptr, ldx, xs_ptr, M,
-                                     out_ptr, _i8_code(I8_TYPES, dtype), ldo, err_ptr, stream), "qkv_i8")
+                                     out_ptr, _i8_code(I8_TYPES, dtype), ldo, err_ptr, stream),
+              "qkv_i8")
 
 
 class FfwdApi:

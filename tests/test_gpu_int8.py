@@ -36,7 +36,10 @@ def mat(w, t, K, bias=None):
 
 def within(got, want, bound):
     err = (got.double() - want).abs()
-    bad = ~(err <= bound)
+    # Past the type's largest value plus half a step, rounding gives infinity.
+    info = torch.finfo(got.dtype)
+    over = torch.isinf(got) & (want * got.sign() + bound >= info.max * (1 + info.eps / 4))
+    bad = ~((err <= bound) | over)
     assert not bad.any(), (int(bad.sum()), float((err / bound).nan_to_num(1e9).max()),
                            bad.nonzero()[:4].tolist())
 
@@ -135,11 +138,13 @@ def test_quantise_special_rows(K, normed):
 
 # ---------------------------------------------------------------- products
 
-# Streaming kernel (up to 8 rows) and tensor-core tiles; lengths on both sides
-# of a tile, a stage and a 16-byte chunk.
-SHAPES = [(1, 64, 16), (1, 1024, 2048), (2, 1, 1), (3, 37, 45), (8, 5000, 530), (8, 10000, 64),
-          (9, 32, 128), (9, 31, 129), (64, 300, 77), (128, 257, 1024), (129, 256, 513),
-          (300, 1003, 771), (257, 4096, 384), (1025, 640, 2100)]
+# Streaming kernel (up to 4 rows), tiles with K split over a cluster (up to 64
+# rows, more for long K) and 256-row tiles; lengths on both sides of a tile, a
+# stage and a 16-byte chunk.
+SHAPES = [(1, 64, 16), (1, 1024, 2048), (2, 1, 1), (3, 37, 45), (4, 5000, 4500), (8, 5000, 530),
+          (8, 10000, 64), (9, 32, 128), (9, 31, 129), (17, 129, 1000), (33, 70, 5000),
+          (64, 300, 77), (100, 200, 4200), (65, 33, 130), (128, 257, 1024), (129, 256, 513),
+          (200, 300, 8300), (300, 1003, 771), (257, 4096, 384), (1025, 640, 2100)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -158,12 +163,12 @@ def test_gemm(M, N, K, dtype):
 def test_gemm_sums_are_exact():
     """The largest sums (every product 127^2, K = 131071) and cancelling ones."""
     K, N = 131071, 48
-    for M in (2, 10):
+    for M in (2, 10, 300):
         x = torch.full((M, K + 1), 127, dtype=torch.int8, device=DEV)
         w = torch.full((N, K + 1), 127, dtype=torch.int8, device=DEV)
         w[1, :K] = -128
         w[2, 1:K:2] = -127
-        one = torch.ones(N, device=DEV)
+        one = torch.ones(max(M, N), device=DEV)
         y = torch.zeros(M, N, device=DEV)
         native.gemm_i8(mat(w, one, K), x.data_ptr(), K + 1, one.data_ptr(), M, y.data_ptr(),
                        "f32", N)
@@ -171,7 +176,7 @@ def test_gemm_sums_are_exact():
         assert torch.equal(y, want)
 
 
-@pytest.mark.parametrize("M", [3, 200])
+@pytest.mark.parametrize("M", [3, 30, 200])
 @pytest.mark.parametrize("dtype,N,ld,off", [("f32", 130, 131, 1), ("bf16", 130, 139, 3),
                                             ("f16", 96, 104, 0), ("bf16", 96, 100, 8)])
 def test_gemm_output_strides(M, dtype, N, ld, off):
@@ -189,7 +194,7 @@ def test_gemm_output_strides(M, dtype, N, ld, off):
     assert (buf[:off] == 7).all()
 
 
-@pytest.mark.parametrize("M,ld", [(5, 96), (5, 97), (333, 96), (333, 97)])
+@pytest.mark.parametrize("M,ld", [(4, 96), (4, 97), (40, 97), (333, 96), (333, 97)])
 def test_gemm_accumulates(M, ld):
     N, K = 96, 300
     x, s = rows(M, K, 4)
@@ -206,7 +211,7 @@ def test_gemm_accumulates(M, ld):
 
 def test_scales_that_are_not_finite_reach_their_row_only():
     M, N, K = 40, 70, 90
-    for m in (4, M):
+    for m in (4, M, 5 * M):
         x, s = rows(m, K, 8)
         w, t = rows(N, K, 9)
         s[1] = float("nan")
@@ -220,8 +225,34 @@ def test_scales_that_are_not_finite_reach_their_row_only():
         within(y[keep], want, bound)
 
 
+@pytest.mark.parametrize("M", [2, 20, 300])
+@pytest.mark.parametrize("kind", ["silu", "gelu", "gelu_tanh"])
+def test_activations_far_out(M, kind):
+    """Arguments up to the ends of f32, infinities and NaN (through the bias):
+    x far to the right, a zero far to the left, +inf kept, NaN kept."""
+    K = 32
+    far = [1e5, 3e18, 1e20, 1e30, 3e38, float("inf")]
+    bias = torch.tensor(far + [-v for v in far[:-1]] + [float("nan"), 0.0, 6.0, -6.0, 12.0, -12.0],
+                        device=DEV)
+    N = bias.numel()
+    x = torch.zeros(M, K, dtype=torch.int8, device=DEV)
+    w = torch.zeros(N, K, dtype=torch.int8, device=DEV)
+    one = torch.ones(max(M, N), device=DEV)
+    y = torch.zeros(M, N, device=DEV)
+    native.gemm_i8(mat(w, one, K, bias), x.data_ptr(), K, one.data_ptr(), M, y.data_ptr(), "f32",
+                   N, act=kind)
+    n = len(far)
+    assert torch.equal(y[:, :n], bias[:n].expand(M, n))
+    assert (y[:, n:2 * n - 1] == 0).all()
+    assert torch.isnan(y[:, 2 * n - 1]).all()
+    near = bias[2 * n:]
+    want, bound = ref.act(near.double(), torch.zeros_like(near.double()), kind, "f32")
+    within(y[:, 2 * n:], want.expand(M, -1), bound.expand(M, -1) + 2.0 ** -60)
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 1024, 512), (2, 33, 100), (7, 7000, 48), (24, 2048, 1024),
-                                   (129, 127, 130), (700, 1111, 1000), (256, 128, 64)])
+                                   (129, 127, 130), (700, 1111, 1000), (256, 128, 64),
+                                   (4, 300, 2000), (50, 130, 4100), (90, 257, 4100)])
 @pytest.mark.parametrize("dtype", list(ref.TYPES))
 def test_gated(M, N, K, dtype):
     x, s = rows(M, K, M)
@@ -255,7 +286,9 @@ def run_qkv(M, K, h, kv, hd, dtype, bias, qn, kn, pos, cos, sin, w, t, x, s, ld=
 @pytest.mark.parametrize("M,K,h,kv,hd", [(1, 256, 2, 1, 128), (7, 1024, 16, 8, 128),
                                          (5, 100, 7, 1, 64), (9, 130, 1, 1, 64),
                                          (130, 384, 3, 3, 128), (600, 904, 14, 2, 64),
-                                         (257, 512, 8, 1, 128)])
+                                         (257, 512, 8, 1, 128), (3, 4096, 2, 1, 64),
+                                         (16, 2100, 1, 1, 128), (33, 700, 3, 1, 64),
+                                         (64, 1024, 16, 8, 128)])
 @pytest.mark.parametrize("dtype", list(ref.TYPES))
 def test_qkv(M, K, h, kv, hd, dtype):
     N = (h + 2 * kv) * hd
@@ -273,7 +306,7 @@ def test_qkv(M, K, h, kv, hd, dtype):
                              1e-6, dtype))
 
 
-@pytest.mark.parametrize("M", [6, 150])
+@pytest.mark.parametrize("M", [5, 40, 150])
 def test_qkv_positions_outside_the_tables(M):
     h, kv, hd, K = 2, 1, 64, 96
     N = (h + 2 * kv) * hd
@@ -359,7 +392,7 @@ def test_feed_forward_block(M, H, I):
     assert cos.min() > 0.998, cos.min()
 
 
-@pytest.mark.parametrize("M", [2, 200])
+@pytest.mark.parametrize("M", [2, 30, 200])
 def test_captured_and_replayed(M):
     """Captured into a graph and replayed on new inputs, with an eager call of
     other rows between: bitwise the eager results."""

@@ -147,6 +147,32 @@ def test_the_plan_is_chosen_per_load(model_root):
         b.close()
 
 
+def test_late_interaction_and_spans(model_root):
+    """Token vectors and span means of 8-bit models."""
+    from golden_util import load_spans
+    from helpers import small_spec
+    from ffwd_b200 import synth
+
+    L = native.lib()
+    d = synth.ensure_model(small_spec("qwen3-late-2l"), model_root)
+    ids = np.arange(100, 140, dtype=np.int32)
+    L.ffwd_b200_set_linear_i8(1)
+    late = native.B200Late(d, gemm_mode="bf16")
+    L.ffwd_b200_set_linear_i8(0)
+    try:
+        vec = late.encode_tokens(ids)
+    finally:
+        late.close()
+    assert cos_rows(vec, of.OracleLate(d).encode_tokens(ids)).min() >= 0.99
+    spec, d, docs, spans, expected = load_spans("qwen3_spans", model_root)
+    m = native.B200Model(d, gemm_mode="bf16", weight_dtype="file", linear_i8=True)
+    try:
+        got = m.encode_spans_batch(docs, spans)
+    finally:
+        m.close()
+    assert cos_rows(got, expected).min() >= 0.99
+
+
 def test_exact_plans_are_refused(model_root):
     spec, d, seqs, _ = load("minilm_f32", model_root)
     for mode in ("f32", "tf32"):

@@ -73,6 +73,8 @@ def qkv(w=None, h=None, **kw):
     (gemm, dict(x_ptr=None), "invalid arguments"),
     (gemm, dict(xs_ptr=None), "invalid arguments"),
     (gemm, dict(M=-2), "invalid arguments"),
+    (gemm, dict(M=(1 << 30) + 1), "invalid arguments"),
+    (quantise, dict(M=(1 << 30) + 1), "invalid arguments"),
     (gemm, dict(ldx=96), "at least 100"),
     (gemm, dict(x_ptr=A + 1), "16-byte aligned"),
     (gemm, dict(y_ptr=None), "invalid arguments"),
