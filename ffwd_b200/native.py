@@ -495,45 +495,46 @@ def i8_heads(n_heads, n_kv_heads, head_dim, pos_ptr, cos_ptr, sin_ptr, n_pos, q_
                                 q_norm_ptr, k_norm_ptr, eps)
 
 
-def _i8_code(table, name):
-    if name not in table:
-        raise FfwdError(f"{name!r} is not one of {', '.join(table)}")
-    return table[name]
+def _i8_fail(what, dtype, act=None):
+    for name, table in ((dtype, I8_TYPES), (act, I8_ACTS)):
+        if name is not None and name not in table:
+            raise FfwdError(f"{what} failed: {name!r} is not one of {', '.join(table)}")
+    raise FfwdError(f"{what} failed: {last_error()}")
 
 
-def _i8_check(rc, what):
-    if rc != 0:
-        raise FfwdError(f"{what} failed: {last_error()}")
-
-
+# (An unknown name goes down as -1, which the call refuses: no check of its own
+# on the way, these calls are counted in microseconds.)
 def quantize_i8(x_ptr, dtype, ldx, q_ptr, ldq, scale_ptr, M, K, norm_ptr=None, eps=0.0, stream=0):
     """Rows to int8 with a scale each, optionally after an RMSNorm with weights
     at norm_ptr."""
-    _i8_check(lib().ffwd_b200_quantize_i8(x_ptr, _i8_code(I8_TYPES, dtype), ldx, norm_ptr, eps,
-                                          q_ptr, ldq, scale_ptr, M, K, stream), "quantize_i8")
+    if (_lib or lib()).ffwd_b200_quantize_i8(x_ptr, I8_TYPES.get(dtype, -1), ldx, norm_ptr, eps,
+                                             q_ptr, ldq, scale_ptr, M, K, stream):
+        _i8_fail("quantize_i8", dtype)
 
 
 def gemm_i8(w, x_ptr, ldx, xs_ptr, M, y_ptr, dtype, ldy, act="none", accumulate=False,
             err_ptr=None, stream=0):
     """y = act(x w^T) (accumulate: y +=) of quantised rows with weights `w` (i8_mat)."""
-    _i8_check(lib().ffwd_b200_gemm_i8(ctypes.byref(w), x_ptr, ldx, xs_ptr, M, y_ptr,
-                                      _i8_code(I8_TYPES, dtype), ldy, _i8_code(I8_ACTS, act),
-                                      int(accumulate), err_ptr, stream), "gemm_i8")
+    if (_lib or lib()).ffwd_b200_gemm_i8(ctypes.byref(w), x_ptr, ldx, xs_ptr, M, y_ptr,
+                                         I8_TYPES.get(dtype, -1), ldy, I8_ACTS.get(act, -1),
+                                         accumulate, err_ptr, stream):
+        _i8_fail("gemm_i8", dtype, act)
 
 
 def gated_i8(gate, up, x_ptr, ldx, xs_ptr, M, h_ptr, dtype, ldh, act="silu", err_ptr=None,
              stream=0):
     """h = act(x gate^T) * (x up^T) of quantised rows."""
-    _i8_check(lib().ffwd_b200_gated_i8(ctypes.byref(gate), ctypes.byref(up), x_ptr, ldx, xs_ptr, M,
-                                       h_ptr, _i8_code(I8_TYPES, dtype), ldh,
-                                       _i8_code(I8_ACTS, act), err_ptr, stream), "gated_i8")
+    if (_lib or lib()).ffwd_b200_gated_i8(ctypes.byref(gate), ctypes.byref(up), x_ptr, ldx, xs_ptr,
+                                          M, h_ptr, I8_TYPES.get(dtype, -1), ldh,
+                                          I8_ACTS.get(act, -1), err_ptr, stream):
+        _i8_fail("gated_i8", dtype, act)
 
 
 def qkv_i8(w, heads, x_ptr, ldx, xs_ptr, M, out_ptr, dtype, ldo, err_ptr=None, stream=0):
     """Fused QKV projection of quantised rows, head norms and rotation included."""
-    _i8_check(lib().ffwd_b200_qkv_i8(ctypes.byref(w), ctypes.byref(heads), x_ptr, ldx, xs_ptr, M,
-                                     out_ptr, _i8_code(I8_TYPES, dtype), ldo, err_ptr, stream),
-              "qkv_i8")
+    if (_lib or lib()).ffwd_b200_qkv_i8(ctypes.byref(w), ctypes.byref(heads), x_ptr, ldx, xs_ptr,
+                                        M, out_ptr, I8_TYPES.get(dtype, -1), ldo, err_ptr, stream):
+        _i8_fail("qkv_i8", dtype)
 
 
 class FfwdApi:
