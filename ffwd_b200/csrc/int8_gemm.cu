@@ -212,45 +212,10 @@ struct Sink {
     }
 };
 
-// 32 integer sums (as bits) to f32.  The conversion instruction runs at a
-// sixteenth of the arithmetic's rate, so sums below 2^22 in magnitude, all but contrived ones, go
-// through the f32 1.5 x 2^23 + sum, whose bits are those of 1.5 x 2^23 plus
-// the sum; the values whose bits leave its binade are converted.
-template <int R>
-__device__ __forceinline__ void to_f32(float (&v)[R][32]) {
-    constexpr int kBias = 0x4B400000;  // 1.5 x 2^23
-    int out = 0;
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const int b = __float_as_int(v[r][i]) + kBias;
-            out |= b ^ 0x4B000000;
-            v[r][i] = __int_as_float(b);
-        }
-    if ((uint32_t)out < 0x800000u) {
-        const float2 down = make_float2(-12582912.0f, -12582912.0f);
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float2 f = add_f32x2(make_float2(v[r][2 * i], v[r][2 * i + 1]), down);
-                v[r][2 * i] = f.x;
-                v[r][2 * i + 1] = f.y;
-            }
-    } else {
-        // volatile: a branch, not both sides and a choice (in twice the registers)
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-                asm volatile("cvt.rn.f32.s32 %0, %1;"
-                             : "=f"(v[r][i])
-                             : "r"(__float_as_int(v[r][i]) - kBias));
-    }
-}
-
-// 32 sums scaled: v = v * s * t + b (b null: no bias).
+// 32 integer sums (as bits) scaled: v = v * s * t + b (b null: no bias).  (The
+// conversion instruction is slow but runs beside the arithmetic; conversions by
+// adding 1.5 x 2^23 to the bits, with a check of their range, measured 10-20 %
+// slower in the gated form.)
 __device__ __forceinline__ void scale32(float (&v)[32], float s, const float *t, const float *b) {
     const float2 s2 = make_float2(s, s);
 #pragma unroll
@@ -258,8 +223,12 @@ __device__ __forceinline__ void scale32(float (&v)[32], float s, const float *t,
         const float4 tv = reinterpret_cast<const float4 *>(t)[i];
         float4 bv = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (b) bv = reinterpret_cast<const float4 *>(b)[i];
-        const float2 a0 = mul_f32x2(make_float2(v[4 * i], v[4 * i + 1]), s2);
-        const float2 a1 = mul_f32x2(make_float2(v[4 * i + 2], v[4 * i + 3]), s2);
+        const float2 a0 = mul_f32x2(make_float2((float)__float_as_int(v[4 * i]),
+                                                (float)__float_as_int(v[4 * i + 1])),
+                                    s2);
+        const float2 a1 = mul_f32x2(make_float2((float)__float_as_int(v[4 * i + 2]),
+                                                (float)__float_as_int(v[4 * i + 3])),
+                                    s2);
         const float2 r0 = fma_f32x2(a0, make_float2(tv.x, tv.y), make_float2(bv.x, bv.y));
         const float2 r1 = fma_f32x2(a1, make_float2(tv.z, tv.w), make_float2(bv.z, bv.w));
         v[4 * i] = r0.x;
@@ -308,17 +277,16 @@ __device__ __forceinline__ void epilogue(const I8Params &p, uint32_t tbase, floa
         for (int u = 0; u < UNITS; ++u) {
             const int c = (g + u * G) * 32;
             const bool in = c < BN && nb * BN + c < p.N;
-            float v[1][32];
+            float v[32];
             if (in) {
-                tmem_ld32(tbase + c, v[0]);
+                tmem_ld32(tbase + c, v);
                 tmem_wait_ld();
             }
             if (u == UNITS - 1) release();
             if (!in) continue;
-            to_f32(v);
-            scale32(v[0], s, cols + u * 32, bias ? bias + u * 32 : nullptr);
-            act32(v[0], p.act);
-            sink.put(v[0], nb * BN + c);
+            scale32(v, s, cols + u * 32, bias ? bias + u * 32 : nullptr);
+            act32(v, p.act);
+            sink.put(v, nb * BN + c);
         }
     } else {
         constexpr int UNITS = NC / 64;
@@ -334,7 +302,6 @@ __device__ __forceinline__ void epilogue(const I8Params &p, uint32_t tbase, floa
             }
             if (k == UNITS - 1) release();
             if (!in) continue;
-            to_f32(v);
             scale32(v[0], s, cols + k * 64, bias ? bias + k * 64 : nullptr);
             act32(v[0], p.act);
             scale32(v[1], s, cols + k * 64 + 32, p.bias2 ? cols + NC + k * 64 + 32 : nullptr);
@@ -371,10 +338,6 @@ __device__ __forceinline__ void epilogue_heads(const I8Params &p, uint32_t tbase
         for (int c = 0; c < HD / 32; ++c) tmem_ld32(tbase + h0 + c * 32, v[c]);
         tmem_wait_ld();
         if (h0 + G * HD >= BN || col0 + G * HD >= p.N) release();  // the last head
-#pragma unroll
-        for (int c = 0; c < HD / 32; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[c][i] = (float)__float_as_int(v[c][i]);
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c)
             scale32(v[c], s, cols + k * HD + c * 32, bias ? bias + k * HD + c * 32 : nullptr);
