@@ -9,6 +9,10 @@
 // thread holds one channel (its scale and bias in registers), a warp stores 32
 // neighbouring channels.
 //
+// Measured (weights in L2): 64 rows of 4096 x 12288 14 us, where the 256-row
+// tiles take 34; of 1024 x 2048 7.8 us; of gate and up of 12288 x 4096 24.6 us
+// (100 MB of weights: 15.6 us at the HBM rate).
+//
 // One tile per CTA.  Warp 0 TMA producer, warp 1 TMEM allocation and MMA issue,
 // warps 2-9 the epilogue: two warpgroups that take turns at 8 rows.
 #include "host_util.h"

@@ -1,7 +1,9 @@
 // 8-bit integer projections of a few rows (see int8.cuh): the weights are read
 // once, straight from memory into registers, and multiplied with the rows by
 // the four-way byte dot product.  Bound by the weights' bytes; a tensor-core
-// tile would spend 256 rows of work on at most 8.
+// tile would spend its rows' work on at most 4.  One row of 4096 x 12288: 8.5 us
+// (weights in L2), of gate and up of 4096 x 1024: 2.6 us, of 24 + 8 heads, K =
+// 1024: 3.5 us.
 //
 // A warp takes R weight rows, a lane 16 bytes of each at a time (512 bytes of
 // a row per load), all of the rows' sums stay in registers (R x MT integers)

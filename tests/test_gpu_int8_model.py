@@ -98,7 +98,7 @@ def test_model(name, mode, wdt, model_root):
 
 @pytest.mark.parametrize("name", ["qwen3_last", "minilm_f32"])
 def test_short_inputs(name, model_root):
-    """Batches of up to 8 tokens (the streaming kernels), and their rows among
+    """Batches of up to 8 tokens (the kernels for few rows), and their rows among
     longer sequences."""
     spec, d, seqs, _ = load(name, model_root)
     short = [np.asarray(s)[:n] for s, n in zip(seqs, (1, 3, 8, 5))]
