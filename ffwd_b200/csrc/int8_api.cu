@@ -89,7 +89,11 @@ int check_out(const void *y, int type, long long ldy, int N) {
     return 0;
 }
 
-int run(int epi, const I8Params &p, const float *const (&extra)[5], cudaStream_t stream) {
+int run(int epi, const I8Params &p, const float *const (&extra)[4], cudaStream_t stream) {
+    if (!aligned4(p.err)) {
+        fail("the error word needs 4-byte alignment");
+        return -1;
+    }
     if (p.M == 0) return 0;
     int dev = 0, sms = 148;
     if (device_info(&dev, &sms)) return -1;

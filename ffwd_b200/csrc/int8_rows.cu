@@ -200,7 +200,7 @@ __device__ __forceinline__ bool put8(float (&x)[8], const float (&g)[8], float i
 // Blocks per SM that the registers allow: the row's values twice (this row's
 // and the next one's, in flight).
 constexpr int min_blocks(int type, bool norm, int w, int nv) {
-    const int regs = 48 + nv * (type == kI8F32 ? 16 : 8) + (norm ? 8 : 0);
+    const int regs = 40 + nv * (type == kI8F32 ? 16 : 8) + (norm ? 8 : 0);
     const int n = 65536 / ((w > 8 ? w : 8) * 32 * regs);
     return n < 1 ? 1 : n > 6 ? 6 : n;
 }

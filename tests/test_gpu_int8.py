@@ -144,7 +144,7 @@ def test_quantise_special_rows(K, normed):
 SHAPES = [(1, 64, 16), (1, 1024, 2048), (2, 1, 1), (3, 37, 45), (4, 5000, 4500), (8, 5000, 530),
           (8, 10000, 64), (9, 32, 128), (9, 31, 129), (17, 129, 1000), (33, 70, 5000),
           (64, 300, 77), (100, 200, 4200), (65, 33, 130), (128, 257, 1024), (129, 256, 513),
-          (200, 300, 8300), (300, 1003, 771), (257, 4096, 384), (1025, 640, 2100)]
+          (20, 40, 3), (300, 40, 1), (300, 1, 20), (200, 300, 8300), (300, 1003, 771), (257, 4096, 384), (1025, 640, 2100)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)

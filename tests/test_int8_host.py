@@ -80,6 +80,7 @@ def qkv(w=None, h=None, **kw):
     (gemm, dict(y_ptr=None), "invalid arguments"),
     (gemm, dict(y_ptr=A + 1), "element alignment"),
     (gemm, dict(ldy=63), "at least 64"),
+    (gemm, dict(err_ptr=A + 2), "error word"),
     (gemm, dict(act="relu"), "is not one of"),
     (gemm, dict(accumulate=True), "only f32"),
     (gated, dict(up=mat(rows=65)), "gate is 64 x 100, up 65 x 100"),
