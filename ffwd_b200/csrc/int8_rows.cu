@@ -201,18 +201,18 @@ __device__ __forceinline__ bool put8(float (&x)[8], const float (&g)[8], float i
 // and the next one's, in flight).
 constexpr int min_blocks(int type, bool norm, int w, int nv) {
     const int regs = 40 + nv * (type == kI8F32 ? 16 : 8) + (norm ? 8 : 0);
-    const int n = 65536 / ((w > 8 ? w : 8) * 32 * regs);
-    return n < 1 ? 1 : n > 6 ? 6 : n;
+    const int n = 65536 / ((w == 1 ? 8 : w) * 32 * regs);
+    return n < 1 ? 1 : n > 12 ? 12 : n;
 }
 
 // W warps per row, each thread holding NV groups of 8 columns (NV = 0: any
-// width, the row read again in each pass).  A block of max(W, 8) warps walks
+// width, the row read again in each pass).  A block of W (8 for W = 1) warps walks
 // over rows, the next row's loads in flight while it works on one.
 template <int TYPE, bool NORM, int COVER, int W, int NV>
-__global__ void __launch_bounds__((W > 8 ? W : 8) * 32, min_blocks(TYPE, NORM, W, NV))
+__global__ void __launch_bounds__((W == 1 ? 8 : W) * 32, min_blocks(TYPE, NORM, W, NV))
     quantize_kernel(const void *x, long long ldx, const float *norm, float eps, int8_t *q,
                     long long ldq, float *s, int M, int K) {
-    constexpr int NW = W > 8 ? W : 8, R = NW / W;  // rows of a block at a time
+    constexpr int NW = W == 1 ? 8 : W, R = NW / W;  // rows of a block at a time
     __shared__ uint32_t sh_max[NW];
     __shared__ float sh_sum[NW], sh_lo[NW];
     griddep_wait();
@@ -463,7 +463,7 @@ struct Args {
 
 template <int TYPE, bool NORM, int COVER, int W, int NV>
 cudaError_t run(const Args &a, cudaStream_t st) {
-    constexpr int NW = W > 8 ? W : 8, R = NW / W;
+    constexpr int NW = W == 1 ? 8 : W, R = NW / W;
     const int grid = std::min((a.M + R - 1) / R, a.num_sms * min_blocks(TYPE, NORM, W, NV));
     return launch_k(quantize_kernel<TYPE, NORM, COVER, W, NV>, dim3(grid), dim3(NW * 32), 0, st,
                     a.x, a.ldx, a.norm, a.eps, a.q, a.ldq, a.s, a.M, a.K);
