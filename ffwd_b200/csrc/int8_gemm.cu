@@ -8,11 +8,11 @@
 // its 128 output rows in TMEM, in two accumulators, so a tile's epilogue runs
 // under the next tile's products.  In the gated form the leader's half of the
 // weight rows are the gate's and its peer's the up projection's, so matching
-// columns meet in one accumulator.  Bound by the 64 KB a pair takes from L2 per
-// 128 bytes of K (12 TB/s over all SMs) and by the power cap, at short K by the
-// epilogue.  Measured: 8192 x 4096 x 12288 265 us (3.1 POPS), gate and up 8192 x
-// 12288 x 4096 550 us (3.0), 8192 x 4096 x 1024 31 us, with GELU 40 us, heads of
-// 32768 x 4096 x 1024 146 us.
+// columns meet in one accumulator.  Bound by the tensor cores at the clock that
+// the power cap leaves and the 64 KB a pair takes from L2 per 128 bytes of K
+// (12.8 TB/s over all SMs), at short K by the epilogue.  Measured: 8192 x 4096 x
+// 12288 254 us (3.2 POPS), gate and up 8192 x 12288 x 4096 506 us (3.3), 8192 x
+// 4096 x 1024 31 us, with GELU 39.5 us, heads of 32768 x 4096 x 1024 144 us.
 //
 // Roles per CTA: warp 0 TMA producer, warp 1 TMEM allocation and (leader) MMA
 // issue, the other warps the epilogue, in warpgroups that split the columns.  No
@@ -82,14 +82,16 @@ __device__ __forceinline__ void tma_load_pair(void *dst, const CUtensorMap *m, u
         : "memory");
 }
 
-// D[tmem, s32] (+)= A * B^T, 8-bit integers.
-__device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                             uint32_t idesc, uint32_t accum) {
+// D[tmem, s32] (+)= A * B^T, 8-bit integers; the operands' descriptors share
+// their upper word.
+__device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo,
+                                             uint32_t hi, uint32_t idesc, uint32_t accum) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accum)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accum)
         : "memory");
 }
 
@@ -543,47 +545,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Cfg<BN, EPI, HD>::T
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (leader && lane == 0) {
+        if (leader) {
             // ---------------------------------------------------------- MMA issuer
+            // The whole warp walks the steps and one elected lane issues, so that
+            // descriptors and counters stay uniform values.  This thread's
+            // instructions set the pace of long products: with a lone lane in the
+            // loop, and descriptors built anew for every product, a step of K took
+            // 609 cycles instead of 580 (512 are the tensor cores').
             constexpr uint32_t IDESC = idesc_i8(2 * BM, BN);
-            int it = 0, lt = 0;
+            const uint64_t desc = smem_desc(smem_u32(smem), 16, 1024, kLayoutSW128);
+            const uint32_t lo = (uint32_t)desc, hi = (uint32_t)(desc >> 32);
+            int lt = 0, s = 0;
+            uint32_t ph = 0;
             bool ok = true;
             int mb, nb;
             for (; ok && tiles.pop(mb, nb); ++lt) {
                 const int a = lt & 1;
                 const uint32_t aph = (lt >> 1) & 1;
-                if (!mbar_wait(&tempty_bar[a], aph ^ 1, p.err, &abort_sh)) {
-                    ok = false;
-                    break;
-                }
+                ok = __all_sync(0xffffffffu, mbar_wait(&tempty_bar[a], aph ^ 1, p.err, &abort_sh));
+                if (!ok) break;
                 tc_fence_after();
                 const uint32_t d = tmem_base + a * BN;
                 for (int kb = 0; kb < k_blocks; ++kb) {
-                    const int s = it % STAGES;
-                    const uint32_t ph = (it / STAGES) & 1;
-                    if (!mbar_wait(&full_bar[s], ph, p.err, &abort_sh)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t sa = smem_u32(smem + s * CF::STAGE);
-                    const uint32_t sb = sa + A_BYTES;
+                    ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[s], ph, p.err, &abort_sh));
+                    if (!ok) break;
+                    if (elect_one_sync()) {
+                        const uint32_t da = lo + s * (CF::STAGE >> 4), db = da + (A_BYTES >> 4);
 #pragma unroll
-                    for (int kk = 0; kk < BK / 32; ++kk)
-                        umma_i8_pair(d, smem_desc(sa + kk * 32, 16, 1024, kLayoutSW128),
-                                     smem_desc(sb + kk * 32, 16, 1024, kLayoutSW128), IDESC,
-                                     (kb | kk) != 0);
-                    umma_commit_pair(&empty_bar[s]);
-                    ++it;
+                        for (int kk = 0; kk < BK / 32; ++kk)
+                            umma_i8_pair(d, da + kk * 2, db + kk * 2, hi, IDESC, (kb | kk) != 0);
+                        umma_commit_pair(&empty_bar[s]);
+                    }
+                    if (++s == STAGES) {
+                        s = 0;
+                        ph ^= 1;
+                    }
                 }
                 if (!ok) break;
-                umma_commit_pair(&tfull_bar[a]);
+                if (elect_one_sync()) umma_commit_pair(&tfull_bar[a]);
             }
             if (!ok) {
-                asm volatile(
-                    "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                        smem_u32(&drain_bar))
-                    : "memory");
+                if (elect_one_sync())
+                    asm volatile(
+                        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                            smem_u32(&drain_bar))
+                        : "memory");
                 mbar_wait(&drain_bar, 0, nullptr, nullptr);
             }
         }
