@@ -12,7 +12,8 @@
 // the power cap leaves and the 64 KB a pair takes from L2 per 128 bytes of K
 // (12.8 TB/s over all SMs), at short K by the epilogue.  Measured: 8192 x 4096 x
 // 12288 254 us (3.2 POPS), gate and up 8192 x 12288 x 4096 506 us (3.3), 8192 x
-// 4096 x 1024 31 us, with GELU 39.5 us, heads of 32768 x 4096 x 1024 144 us.
+// 4096 x 1024 31 us, with GELU 39.5 us, heads of 32768 x 4096 x 1024 146 us,
+// of 8192 x 6144 x 4096 145 us.
 //
 // Roles per CTA: warp 0 TMA producer, warp 1 TMEM allocation and (leader) MMA
 // issue, the other warps the epilogue, in warpgroups that split the columns.  No
@@ -408,32 +409,33 @@ __device__ __forceinline__ void epilogue_heads(const I8Params &p, uint32_t tbase
     }
 }
 
-// Tiles of one SM pair, in order.  Head form: a run of neighbouring tiles, row
-// blocks outermost, so that the rotary rows change seldom.  Otherwise the pairs
-// take turns over groups of kRaster row blocks, columns outermost within a
-// group: the pairs' tiles of one moment then share both operands (with row
-// blocks outermost they would share one row block and read 74 different weight
-// tiles, all of a large matrix per row block).
+// Tiles of one SM pair, in order.  The pairs take turns over groups of kRaster
+// row blocks, columns outermost within a group: the pairs' tiles of one moment
+// then share both operands (with row blocks outermost they would share one row
+// block and read 74 different weight tiles, all of a large matrix per row block).
+// `runs` (head form, K <= kRunK): a pair takes a run of neighbouring tiles, row
+// blocks outermost, so that the rotary rows, 3000 cycles to fetch, change seldom;
+// but the pairs are then at 74 places of the weights and hold 74 row blocks,
+// which L2 keeps only while K is short, and a longer K hides the rows' fetch.
+// Heads with runs and in turns: 32768 x 4096 x 1024 146 and 189 us, 32768 x 6144
+// x 2048 309 and 340, 8192 x 6144 x 2560 94 and 97, 32768 x 6144 x 2560 400 and
+// 364, 16384 x 6144 x 4096 380 and 278, 16384 x 7168 x 5120 580 and 411.
 constexpr int kRaster = 8;
+constexpr int kRunK = 2048;
 
-template <int EPI>
 struct Tiles {
+    bool runs;
     int m_blocks, n_blocks, next, end, step;
-    __device__ Tiles(int mb, int nb, int pair, int n_pairs) : m_blocks(mb), n_blocks(nb) {
+    __device__ Tiles(int mb, int nb, int pair, int n_pairs, bool runs_)
+        : runs(runs_), m_blocks(mb), n_blocks(nb) {
         const int total = mb * nb;
-        if (EPI == kI8Heads) {
-            next = (int)((long long)total * pair / n_pairs);
-            end = (int)((long long)total * (pair + 1) / n_pairs);
-            step = 1;
-        } else {
-            next = pair;
-            end = total;
-            step = n_pairs;
-        }
+        next = runs ? (int)((long long)total * pair / n_pairs) : pair;
+        end = runs ? (int)((long long)total * (pair + 1) / n_pairs) : total;
+        step = runs ? 1 : n_pairs;
     }
     __device__ __forceinline__ bool pop(int &mb, int &nb) {
         if (next >= end) return false;
-        if (EPI == kI8Heads) {
+        if (runs) {
             mb = next / n_blocks;
             nb = next % n_blocks;
         } else {
@@ -478,7 +480,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Cfg<BN, EPI, HD>::T
     const int pair = blockIdx.x >> 1;
     const int n_pairs = gridDim.x >> 1;
 
-    Tiles<EPI> tiles(m_blocks, n_blocks, pair, n_pairs);
+    Tiles tiles(m_blocks, n_blocks, pair, n_pairs, EPI == kI8Heads && p.K <= kRunK);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
