@@ -11,9 +11,9 @@
 // columns meet in one accumulator.  Bound by the tensor cores at the clock that
 // the power cap leaves and the 64 KB a pair takes from L2 per 128 bytes of K
 // (12.8 TB/s over all SMs), at short K by the epilogue.  Measured: 8192 x 4096 x
-// 12288 254 us (3.2 POPS), gate and up 8192 x 12288 x 4096 506 us (3.3), 8192 x
-// 4096 x 1024 31 us, with GELU 39.5 us, heads of 32768 x 4096 x 1024 146 us,
-// of 8192 x 6144 x 4096 145 us.
+// 12288 254 us (3.2 POPS), gate and up 8192 x 12288 x 4096 485 us (3.4), 8192 x
+// 4096 x 1024 31 us, with GELU 39.5 us, heads of 32768 x 4096 x 1024 145 us, of
+// 8192 x 6144 x 4096 143 us.
 //
 // Roles per CTA: warp 0 TMA producer, warp 1 TMEM allocation and (leader) MMA
 // issue, the other warps the epilogue, in warpgroups that split the columns.  No
@@ -409,43 +409,61 @@ __device__ __forceinline__ void epilogue_heads(const I8Params &p, uint32_t tbase
     }
 }
 
-// Tiles of one SM pair, in order.  The pairs take turns over groups of kRaster
-// row blocks, columns outermost within a group: the pairs' tiles of one moment
-// then share both operands (with row blocks outermost they would share one row
-// block and read 74 different weight tiles, all of a large matrix per row block).
-// `runs` (head form, K <= kRunK): a pair takes a run of neighbouring tiles, row
-// blocks outermost, so that the rotary rows, 3000 cycles to fetch, change seldom;
-// but the pairs are then at 74 places of the weights and hold 74 row blocks,
-// which L2 keeps only while K is short, and a longer K hides the rows' fetch.
-// Heads with runs and in turns: 32768 x 4096 x 1024 146 and 189 us, 32768 x 6144
-// x 2048 309 and 340, 8192 x 6144 x 2560 94 and 97, 32768 x 6144 x 2560 400 and
-// 364, 16384 x 6144 x 4096 380 and 278, 16384 x 7168 x 5120 580 and 411.
+// Tiles of one SM pair, in order.  The pairs take turns over groups of row
+// blocks, columns outermost within a group: the pairs' tiles of one moment then
+// share both operands (with row blocks outermost they would share one row block
+// and read 74 different weight tiles, all of a large matrix per row block).  A
+// group is 8 blocks.  Gate and up weights that do not stay in L2 are read once a
+// group, so there it is as many as 32 MB of quantised rows allow, up to 32 (8192 x
+// 12288 x 4096 with 8 and 32 blocks 510 and 485 us, 32768 rows of it 2210 and
+// 2120; plain products of 4096 columns lose 1-2 % by larger groups).
+// Head form, K <= kRunK: a pair takes a run of neighbouring tiles, row blocks
+// outermost, so that the rotary rows, 3000 cycles to fetch, change seldom; but
+// the pairs are then at 74 places of the weights and hold 74 row blocks, which L2
+// keeps only while K is short, and a longer K hides the rows' fetch.  Heads in
+// runs and in turns: 32768 x 4096 x 1024 146 and 189 us, 32768 x 6144 x 2048 309
+// and 340, 8192 x 6144 x 2560 94 and 97, 32768 x 6144 x 2560 400 and 364, 16384 x
+// 6144 x 4096 380 and 278, 16384 x 7168 x 5120 580 and 411.
 constexpr int kRaster = 8;
 constexpr int kRunK = 2048;
+constexpr long long kKeptWeights = 24ll << 20;  // bytes
 
+int raster_group(const I8Params &p) {
+    if (2ll * p.N * p.K <= kKeptWeights) return kRaster;
+    return (int)std::max<long long>(kRaster, std::min(32ll, (32ll << 20) / (2ll * BM * p.K)));
+}
+
+// (What the launch's parameters give is computed anew: the head form's epilogue
+// has no registers left to keep it in.)
+template <int EPI, int TN>
 struct Tiles {
-    bool runs;
-    int m_blocks, n_blocks, next, end, step;
-    __device__ Tiles(int mb, int nb, int pair, int n_pairs, bool runs_)
-        : runs(runs_), m_blocks(mb), n_blocks(nb) {
-        const int total = mb * nb;
-        next = runs ? (int)((long long)total * pair / n_pairs) : pair;
-        end = runs ? (int)((long long)total * (pair + 1) / n_pairs) : total;
-        step = runs ? 1 : n_pairs;
+    const I8Params &p;
+    const int &group_rows;
+    int next, end;
+    __device__ __forceinline__ int m_blocks() const { return (p.M + 2 * BM - 1) / (2 * BM); }
+    __device__ __forceinline__ int n_blocks() const { return (p.N + TN - 1) / TN; }
+    __device__ __forceinline__ int pairs() const { return gridDim.x >> 1; }
+    __device__ __forceinline__ bool runs() const { return EPI == kI8Heads && p.K <= kRunK; }
+    __device__ Tiles(const I8Params &p_, const int &group_rows_) : p(p_), group_rows(group_rows_) {
+        const int total = m_blocks() * n_blocks(), pair = blockIdx.x >> 1;
+        next = runs() ? (int)((long long)total * pair / pairs()) : pair;
+        end = runs() ? (int)((long long)total * (pair + 1) / pairs()) : total;
     }
     __device__ __forceinline__ bool pop(int &mb, int &nb) {
         if (next >= end) return false;
-        if (runs) {
-            mb = next / n_blocks;
-            nb = next % n_blocks;
+        if (runs()) {
+            mb = next / n_blocks();
+            nb = next % n_blocks();
+            ++next;
         } else {
-            const int group = next / (kRaster * n_blocks);
-            const int rows = min(kRaster, m_blocks - group * kRaster);
-            const int r = next - group * kRaster * n_blocks;
-            mb = group * kRaster + r % rows;
+            const int R = EPI == kI8Gated ? group_rows : kRaster;
+            const int group = next / (R * n_blocks());
+            const int rows = min(R, m_blocks() - group * R);
+            const int r = next - group * R * n_blocks();
+            mb = group * R + r % rows;
             nb = r / rows;
+            next += pairs();
         }
-        next += step;
         return true;
     }
 };
@@ -454,7 +472,8 @@ template <int BN, int EPI, int HD>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Cfg<BN, EPI, HD>::THREADS), 1)
     i8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmB2,
-                   const __grid_constant__ CUtensorMap tmOut, const I8Params p, const int tma_out) {
+                   const __grid_constant__ CUtensorMap tmOut, const I8Params p, const int tma_out,
+                   const int group_rows) {
     extern __shared__ uint8_t smem_raw[];
     using CF = Cfg<BN, EPI, HD>;
     constexpr int STAGES = CF::STAGES, GROUPS = CF::GROUPS;
@@ -474,13 +493,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Cfg<BN, EPI, HD>::T
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
 
     constexpr int TN = EPI == kI8Gated ? BN / 2 : BN;  // output columns per tile
-    const int m_blocks = (p.M + 2 * BM - 1) / (2 * BM);
-    const int n_blocks = (p.N + TN - 1) / TN;
     const int k_blocks = (p.K + BK - 1) / BK;
-    const int pair = blockIdx.x >> 1;
-    const int n_pairs = gridDim.x >> 1;
-
-    Tiles tiles(m_blocks, n_blocks, pair, n_pairs, EPI == kI8Heads && p.K <= kRunK);
+    Tiles<EPI, TN> tiles(p, group_rows);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
@@ -740,7 +754,8 @@ int launch(const I8Params &p, int num_sms, cudaStream_t stream) {
     const long long tiles = (long long)((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + TN - 1) / TN);
     const int grid = (int)std::min<long long>(2 * tiles, num_sms & ~1);
     LAUNCH(launch_k(i8_gemm_kernel<BN, EPI, HD>, dim3(grid), dim3(Cfg<BN, EPI, HD>::THREADS), (Cfg<BN, EPI, HD>::SMEM), stream,
-                    ma, mb, mb2, mo, p, tma ? 1 : 0));
+                    ma, mb, mb2, mo, p, tma ? 1 : 0,
+                    EPI == kI8Gated ? raster_group(p) : kRaster));
     return 0;
 }
 

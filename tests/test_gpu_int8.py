@@ -306,6 +306,34 @@ def test_qkv(M, K, h, kv, hd, dtype):
                              1e-6, dtype))
 
 
+@pytest.mark.parametrize("M,K,h,kv,hd", [(2400, 2064, 4, 1, 128), (2400, 2048, 4, 1, 128),
+                                         (2100, 2300, 7, 2, 64), (5000, 160, 2, 2, 128)])
+def test_qkv_over_many_tiles(M, K, h, kv, hd):
+    """More than one group of row blocks, the last of them short, on both sides of
+    the K where the order of the tiles changes."""
+    N = (h + 2 * kv) * hd
+    x, s = rows(M, K, 3)
+    w, t = rows(N, K, 4)
+    cos, sin = tables(M, hd)
+    pos = torch.randperm(M, device=DEV, generator=gen(5)).int()
+    qn = 1.0 + 0.2 * torch.randn(hd, device=DEV, generator=gen(6))
+    out = run_qkv(M, K, h, kv, hd, "bf16", None, qn, None, pos, cos, sin, w, t, x, s)
+    within(out, *ref.qkv(x[:, :K], s, w[:, :K], t, None, h, kv, hd, pos, cos, sin, qn, None, 1e-6,
+                         "bf16"))
+
+
+@pytest.mark.parametrize("M,N,K", [(2300, 2600, 5000), (9000, 1600, 8300), (8600, 6200, 2048)])
+def test_gated_of_weights_past_the_cache(M, N, K):
+    """Groups of up to 26, 15 and 32 row blocks, the last of them short."""
+    x, s = rows(M, K, 7)
+    wg, tg = rows(N, K, 8)
+    wu, tu = rows(N, K, 9)
+    h = torch.full((M, N), float("nan"), dtype=torch.float16, device=DEV)
+    native.gated_i8(mat(wg, tg, K), mat(wu, tu, K), x.data_ptr(), x.stride(0), s.data_ptr(), M,
+                    h.data_ptr(), "f16", N)
+    within(h, *ref.gated(x[:, :K], s, wg[:, :K], tg, None, wu[:, :K], tu, None, "silu", "f16"))
+
+
 @pytest.mark.parametrize("M", [5, 40, 150])
 def test_qkv_positions_outside_the_tables(M):
     h, kv, hd, K = 2, 1, 64, 96
