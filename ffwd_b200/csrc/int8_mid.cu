@@ -69,13 +69,15 @@ __device__ __forceinline__ int load_peer(uint32_t addr, uint32_t rank) {
     return v;
 }
 
-__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+// (The operands' descriptors share their upper word.)
+__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi,
                                         uint32_t idesc, uint32_t accum) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accum)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accum)
         : "memory");
 }
 
@@ -161,33 +163,34 @@ __global__ void __launch_bounds__(kThreads)
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t IDESC = idesc_i8(BC, T);
-            int it = 0;
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const int s = it % STAGES;
-                if (!mbar_wait(&full_bar[s], (it / STAGES) & 1, p.err, &abort_sh)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t sw = smem_u32(smem + s * CF::STAGE);
-                const uint32_t sx = sw + CF::MATS * CF::W_BYTES;
+        // The whole warp walks the steps and one elected lane issues, so that
+        // descriptors and counters stay uniform values.
+        constexpr uint32_t IDESC = idesc_i8(BC, T);
+        const uint64_t desc = smem_desc(smem_u32(smem), 16, 1024, kLayoutSW128);
+        const uint32_t lo = (uint32_t)desc, hi = (uint32_t)(desc >> 32);
+        int s = 0;
+        uint32_t ph = 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[s], ph, p.err, &abort_sh));
+            if (!ok) break;
+            if (elect_one_sync()) {
+                const uint32_t dw = lo + s * (CF::STAGE >> 4);
+                const uint32_t dx = dw + CF::MATS * (CF::W_BYTES >> 4);
 #pragma unroll
-                for (int kk = 0; kk < BK / 32; ++kk) {
-                    const uint64_t xd = smem_desc(sx + kk * 32, 16, 1024, kLayoutSW128);
+                for (int kk = 0; kk < BK / 32; ++kk)
 #pragma unroll
                     for (int m = 0; m < CF::MATS; ++m)
-                        umma_i8(tmem + m * T,
-                                smem_desc(sw + m * CF::W_BYTES + kk * 32, 16, 1024, kLayoutSW128),
-                                xd, IDESC, (it | kk) != 0);
-                }
+                        umma_i8(tmem + m * T, dw + m * (CF::W_BYTES >> 4) + kk * 2, dx + kk * 2,
+                                hi, IDESC, kb != kb0 || kk != 0);
                 umma_commit(&empty_bar[s]);
             }
-            umma_commit(&done_bar);
-            if (!mbar_wait(&done_bar, 0, p.err, nullptr)) ok = false;
+            if (++s == STAGES) {
+                s = 0;
+                ph ^= 1;
+            }
         }
-        __syncwarp();
+        if (elect_one_sync()) umma_commit(&done_bar);
+        if (!mbar_wait(&done_bar, 0, p.err, nullptr)) ok = false;
     }
     // Every thread learns whether the products are complete (this also holds the
     // epilogue back until they are).
