@@ -9,8 +9,8 @@
 // thread holds one channel (its scale and bias in registers), a warp stores 32
 // neighbouring channels.
 //
-// Measured (weights in L2): 64 rows of 4096 x 12288 14 us, where the 256-row
-// tiles take 34; of 1024 x 2048 7.8 us; of gate and up of 12288 x 4096 24.6 us
+// Measured (weights in L2): 64 rows of 4096 x 12288 12 us, where the 256-row
+// tiles take 28; of 1024 x 2048 6.1 us; of gate and up of 12288 x 4096 24 us
 // (100 MB of weights: 15.6 us at the HBM rate).
 //
 // One tile per CTA.  Warp 0 TMA producer, warp 1 TMEM allocation and MMA issue,
@@ -22,6 +22,7 @@
 #include "ptx.cuh"
 
 #include <algorithm>
+#include <atomic>
 
 namespace fb {
 namespace {
@@ -399,26 +400,68 @@ int launch_t(const I8Params &p, int split, cudaStream_t stream) {
     return launch<EPI, 64, HD>(p, split, stream);
 }
 
+// Clusters of `size` CTAs (4 or 8) that the device runs at a time, one CTA to an
+// SM: the SMs of a GPC that make up no whole cluster stay idle (here 33 clusters
+// of 4 and 15 of 8, not 37 and 18).  One too many costs a second round: 2048
+// channels, K = 4096 in 16 clusters of 8 12.0 us, in 16 of 4 6.5 us.
+int resident_clusters(int size, int num_sms) {
+    static std::atomic<int> known[64][2];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    std::atomic<int> *slot = dev < 64 ? &known[dev][size == 8] : nullptr;
+    int n = slot ? slot->load(std::memory_order_relaxed) : 0;
+    if (n > 0) return n;
+    constexpr auto kern = i8_mid_kernel<kI8Store, 64, 0>;
+    constexpr int smem = Cfg<kI8Store, 64>::SMEM;
+    static_assert(2 * smem > 227 * 1024, "one CTA to an SM, as all variants are");
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(num_sms / size * size);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = size;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (set_smem_once<kern>(smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        return 0;  // no such clusters: K is split less
+    }
+    if (slot) slot->store(n, std::memory_order_relaxed);
+    return n;
+}
+
 }  // namespace
 
 // Up to 64 rows.  More, where K is long: the 256-row tiles of int8_gemm.cu do
-// not split it (4096 channels, K = 12288: 128 rows 16.6 us here, 34.3 there; 256
-// rows 25.5 and 34.6; 1024 channels, K = 2048, 128 rows: 10.1 and 8.8; heads of
-// K = 4096, 128 rows: 23.5 and 17.2), unless they fill the SMs.
+// not split it (4096 channels, K = 12288: 128 rows 14.6 us here, 28.2 there; 256
+// rows 21.1 and 28.2; 1024 channels, K = 2048, 128 rows: 9.8 and 7.5; heads of
+// K = 4096, 128 rows: 28.9 and 15.5).  Over 128 rows only where the tiles leave
+// SMs to split K over (8192 channels, K = 8192, 256 rows: 26.3 and 21.3).
 bool i8_mid_fits(int epi, const I8Params &p, int num_sms) {
     if (p.M <= 64) return true;
     if (epi == kI8Heads) return false;
     if (p.M <= 128) return p.K >= 4096;
     const long long cols = epi == kI8Gated ? 2ll * p.N : p.N;
-    return p.M <= 256 && p.K >= 8192 && (cols + 255) / 256 * 4 <= num_sms;
+    return p.M <= 256 && p.K >= 8192 && (cols + 255) / 256 * 8 <= num_sms;
 }
 
 int i8_mid_run(int epi, const I8Params &p, int num_sms, cudaStream_t stream) {
-    // Split K until the CTAs fill the SMs, as long as each keeps two stages' worth.
+    // K is split while all clusters run at a time and each CTA keeps two steps;
+    // in eight, only where it keeps 4 (up to 32 rows; 1024 channels, K = 4096:
+    // 6.2 us against 6.5 of four, K = 2560: 6.0 and 5.6) or 8 (1024 channels, 64
+    // rows, K = 4096: 7.9 and 7.4, K = 12288: 10.1 and 11.0).
     const long long tiles = (p.N + BC - 1ll) / BC * ((p.M + 127) / 128);
     const int k_blocks = (p.K + BK - 1) / BK;
     int split = 1;
-    while (split < 8 && tiles * split * 2 <= num_sms && k_blocks >= 4 * split) split *= 2;
+    for (int c = 2; c <= 8; c *= 2) {
+        const int steps = c < 8 ? 2 : p.M <= 32 ? 4 : 8;
+        if (tiles * c > num_sms || k_blocks < steps * c) break;
+        if (c > 2 && tiles > resident_clusters(c, num_sms)) break;
+        split = c;
+    }
     switch (epi) {
     case kI8Store: return launch_t<kI8Store, 0>(p, split, stream);
     case kI8Gated: return launch_t<kI8Gated, 0>(p, split, stream);
