@@ -435,17 +435,26 @@ int resident_clusters(int size, int num_sms) {
 
 }  // namespace
 
+// Channel tiles times row blocks.
+long long mid_tiles(int epi, const I8Params &p) {
+    const int rows = epi == kI8Heads ? 64 : 128;
+    return (p.N + BC - 1ll) / BC * ((p.M + rows - 1) / rows);
+}
+
 // Up to 64 rows.  More, where K is long: the 256-row tiles of int8_gemm.cu do
-// not split it (4096 channels, K = 12288: 128 rows 14.6 us here, 28.2 there; 256
-// rows 21.1 and 28.2; 1024 channels, K = 2048, 128 rows: 9.8 and 7.5; heads of
-// K = 4096, 128 rows: 28.9 and 15.5).  Over 128 rows only where the tiles leave
-// SMs to split K over (8192 channels, K = 8192, 256 rows: 26.3 and 21.3).
+// not split it (4096 channels, K = 12288: 128 rows 14.6 us here, 28.2 there; K =
+// 4096: 10.5 and 12.3, K = 2560: 9.6 and 9.3; gate and up of 2048 channels, K =
+// 8192: 16.3 and 19.8, of 4096 channels, K = 4096: 14.7 and 13.1).  Heads over 64
+// rows, and all over 128, only where the tiles leave SMs to split K over (K =
+// 8192, 256 rows: 4096 channels 17.0 and 20.2, 8192 channels 26.3 and 21.3, gate
+// and up of 2048 17.5 and 19.7, of 2560 24.3 and 20.1; K = 4096, 128 rows: 12
+// heads 10.4 and 14.6, 32 heads 20.5 and 14.8).
 bool i8_mid_fits(int epi, const I8Params &p, int num_sms) {
     if (p.M <= 64) return true;
-    if (epi == kI8Heads) return false;
-    if (p.M <= 128) return p.K >= 4096;
-    const long long cols = epi == kI8Gated ? 2ll * p.N : p.N;
-    return p.M <= 256 && p.K >= 8192 && (cols + 255) / 256 * 8 <= num_sms;
+    if (epi == kI8Heads) return p.M <= 128 && p.K >= 2048 && mid_tiles(epi, p) * 4 <= num_sms;
+    if (p.M <= 128) return p.K >= (epi == kI8Gated ? 8192 : 4096);
+    const int halves = epi == kI8Gated ? 4 : 2;
+    return p.M <= 256 && p.K >= 8192 && mid_tiles(epi, p) * halves <= num_sms;
 }
 
 int i8_mid_run(int epi, const I8Params &p, int num_sms, cudaStream_t stream) {
@@ -453,7 +462,7 @@ int i8_mid_run(int epi, const I8Params &p, int num_sms, cudaStream_t stream) {
     // in eight, only where it keeps 4 (up to 32 rows; 1024 channels, K = 4096:
     // 6.2 us against 6.5 of four, K = 2560: 6.0 and 5.6) or 8 (1024 channels, 64
     // rows, K = 4096: 7.9 and 7.4, K = 12288: 10.1 and 11.0).
-    const long long tiles = (p.N + BC - 1ll) / BC * ((p.M + 127) / 128);
+    const long long tiles = mid_tiles(epi, p);
     const int k_blocks = (p.K + BK - 1) / BK;
     int split = 1;
     for (int c = 2; c <= 8; c *= 2) {

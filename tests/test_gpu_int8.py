@@ -307,10 +307,12 @@ def test_qkv(M, K, h, kv, hd, dtype):
 
 
 @pytest.mark.parametrize("M,K,h,kv,hd", [(2400, 2064, 4, 1, 128), (2400, 2048, 4, 1, 128),
-                                         (2100, 2300, 7, 2, 64), (5000, 160, 2, 2, 128)])
+                                         (2100, 2300, 7, 2, 64), (5000, 160, 2, 2, 128),
+                                         (65, 2048, 8, 2, 128), (127, 4100, 3, 1, 64),
+                                         (128, 9000, 1, 1, 128)])
 def test_qkv_over_many_tiles(M, K, h, kv, hd):
     """More than one group of row blocks, the last of them short, on both sides of
-    the K where the order of the tiles changes."""
+    the K where the order of the tiles changes; two row blocks of a split K."""
     N = (h + 2 * kv) * hd
     x, s = rows(M, K, 3)
     w, t = rows(N, K, 4)
@@ -332,6 +334,17 @@ def test_gated_of_weights_past_the_cache(M, N, K):
     native.gated_i8(mat(wg, tg, K), mat(wu, tu, K), x.data_ptr(), x.stride(0), s.data_ptr(), M,
                     h.data_ptr(), "f16", N)
     within(h, *ref.gated(x[:, :K], s, wg[:, :K], tg, None, wu[:, :K], tu, None, "silu", "f16"))
+
+
+@pytest.mark.parametrize("M,N,K", [(7, 1950, 2600), (33, 2048, 9000), (16, 4250, 1100),
+                                   (130, 1100, 8200), (100, 4500, 4200)])
+def test_gemm_of_few_rows_and_many_clusters(M, N, K):
+    """Numbers of channel tiles on both sides of the clusters that fit at a time."""
+    x, s = rows(M, K, 1)
+    w, t = rows(N, K, 2)
+    y = torch.full((M, N), float("nan"), device=DEV)
+    native.gemm_i8(mat(w, t, K), x.data_ptr(), x.stride(0), s.data_ptr(), M, y.data_ptr(), "f32", N)
+    within(y, *ref.gemm(x[:, :K], s, w[:, :K], t, None, "none", "f32"))
 
 
 @pytest.mark.parametrize("M", [5, 40, 150])
