@@ -270,11 +270,14 @@ cudaError_t run(int epi, const I8Params &p, int num_sms, cudaStream_t st) {
 
 }  // namespace
 
-// Up to 2 rows; 3 and 4 while the weights are under 16 MB (4096 x 12288 with 4
-// rows: 21 us against 12.5 of int8_mid.cu; 8192 x 1024: 4.0 against 5.9).
+// Up to 2 rows; 3 and 4 while K and the weights are small (4 rows of 8192 x 1024
+// 3.9 us against 5.5 of int8_mid.cu, of 1024 x 2048 4.5 and 5.3; of 1024 x 4096
+// 7.7 and 6.3, of 4096 x 12288 21 and 10.9; of 24 + 8 heads, K = 1024 6.2 and 7.0,
+// K = 2048 8.8 and 7.5).
 bool i8_vec_fits(int epi, const I8Params &p) {
     if (p.M <= 2) return true;
-    return p.M <= 4 && (long long)p.N * p.K * (epi == kI8Gated ? 2 : 1) <= 16 << 20;
+    return p.M <= 4 && p.K <= (epi == kI8Heads ? 1024 : 2048) &&
+           (long long)p.N * p.K * (epi == kI8Gated ? 2 : 1) <= 16 << 20;
 }
 
 int i8_vec_launch(int epi, const I8Params &p, int num_sms, cudaStream_t stream) {
