@@ -45,6 +45,7 @@ struct Cfg {
     static constexpr int OFF_VALUES = MATS * T * BC * 4;
     static_assert(OFF_VALUES + (EPI == kI8Heads ? T * (BC + 4) * 4 : 0) <= STAGES * STAGE,
                   "the sums fit the stages");
+    static_assert(2 * SMEM > 227 * 1024, "one CTA to an SM (resident_clusters)");
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -413,7 +414,6 @@ int resident_clusters(int size, int num_sms) {
     if (n > 0) return n;
     constexpr auto kern = i8_mid_kernel<kI8Store, 64, 0>;
     constexpr int smem = Cfg<kI8Store, 64>::SMEM;
-    static_assert(2 * smem > 227 * 1024, "one CTA to an SM, as all variants are");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(num_sms / size * size);
     cfg.blockDim = dim3(kThreads);
