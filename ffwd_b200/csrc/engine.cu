@@ -44,7 +44,7 @@ namespace {
 
 int g_gemm_mode = 0;         // 0 f32, 1 tf32, 2 bf16, 3 16f (reference default: f32)
 int g_weight_override = -1;  // -1 file dtype, 0 f32, 1 bf16, 2 f16
-bool g_linear_i8 = false;    // projections in 8-bit integers (16-bit plans)
+std::atomic<bool> g_linear_i8{false};  // 8-bit projections, for loads without a choice of their own
 std::vector<int> g_devices;
 bool g_devices_set = false;
 int g_max_tokens = 262144;
@@ -1428,7 +1428,22 @@ bool has_late_projection(const std::string &dir) {
            stat((dir + "/1_Dense/model.safetensors").c_str(), &st) == 0;
 }
 
-ffwd_b200_ctx *load_ctx(const char *model_dir);
+// linear_i8: projections in 8-bit integers.
+ffwd_b200_ctx *load_ctx(const char *model_dir, bool linear_i8);
+ffwd_b200_ctx *load_pooled(const char *model_dir, bool linear_i8);
+ffwd_b200_late_ctx *load_late(const char *model_dir, bool linear_i8);
+
+// A load's choice of projections: 1 8-bit, 0 the 16-bit or exact plan's, -1 the
+// process's switch.  The switch is read here, once: a load that runs while
+// another thread writes it has one plan throughout.
+bool linear_choice(int linear_i8, bool *on) {
+    if (linear_i8 < -1 || linear_i8 > 1) {
+        fail("linear_i8 must be -1, 0 or 1 (got %d)", linear_i8);
+        return false;
+    }
+    *on = linear_i8 < 0 ? g_linear_i8.load() : linear_i8 != 0;
+    return true;
+}
 
 }  // namespace
 }  // namespace fb
@@ -1487,8 +1502,22 @@ FFWD_B200_API const char *ffwd_b200_last_error(void) { return t_err.c_str(); }
 FFWD_B200_API long long ffwd_b200_launch_count(void) { return g_launches.load(); }
 
 FFWD_B200_API ffwd_b200_ctx_t *ffwd_b200_load(const char *model_dir) {
+    return ffwd_b200_load_linear(model_dir, -1);
+}
+
+FFWD_B200_API ffwd_b200_ctx_t *ffwd_b200_load_linear(const char *model_dir, int linear_i8) {
     t_err.clear();
-    if (!model_dir) return nullptr;
+    bool i8 = false;
+    if (!model_dir || !linear_choice(linear_i8, &i8)) return nullptr;
+    return load_pooled(model_dir, i8);
+}
+
+}  // extern "C"
+
+namespace fb {
+namespace {
+
+ffwd_b200_ctx *load_pooled(const char *model_dir, bool linear_i8) {
     // A 1_Dense head makes the directory a late-interaction model, which is not
     // a pooled embedding model (libffwd/model.c:308-314).
     if (has_late_projection(model_dir)) {
@@ -1497,15 +1526,10 @@ FFWD_B200_API ffwd_b200_ctx_t *ffwd_b200_load(const char *model_dir) {
              model_dir);
         return nullptr;
     }
-    return load_ctx(model_dir);
+    return load_ctx(model_dir, linear_i8);
 }
 
-}  // extern "C"
-
-namespace fb {
-namespace {
-
-ffwd_b200_ctx *load_ctx(const char *model_dir) {
+ffwd_b200_ctx *load_ctx(const char *model_dir, bool linear_i8) {
     auto hm = std::make_unique<HostModel>();
     std::string err;
     if (!parse_model_config(model_dir, hm->cfg, err) || !hm->st.open(model_dir, err)) {
@@ -1583,7 +1607,7 @@ ffwd_b200_ctx *load_ctx(const char *model_dir) {
         prec = 0;
         f16 = store == 2 || (store == 0 && g_gemm_mode == 3);
     }
-    if (g_linear_i8) {
+    if (linear_i8) {
         if (prec != 0) {
             fail("8-bit projections go with a 16-bit plan (--gpu-gemm-mode bf16 or 16f, or 16-bit "
                  "decoder weights)");
@@ -1594,7 +1618,7 @@ ffwd_b200_ctx *load_ctx(const char *model_dir) {
             return nullptr;
         }
     }
-    hm->i8 = g_linear_i8;
+    hm->i8 = linear_i8;
     hm->prec = prec;
     hm->store = store;
     hm->f16 = f16;
@@ -2206,14 +2230,7 @@ int late_check_docs(const int *const *doc_ids, const int *n_tokens, const int *c
     return 0;
 }
 
-}  // namespace
-}  // namespace fb
-
-extern "C" {
-
-FFWD_B200_API ffwd_b200_late_ctx_t *ffwd_b200_late_load(const char *model_dir) {
-    t_err.clear();
-    if (!model_dir) return nullptr;
+ffwd_b200_late_ctx *load_late(const char *model_dir, bool linear_i8) {
     if (!has_late_projection(model_dir)) {
         fail("late load %s: missing 1_Dense projection", model_dir);
         return nullptr;
@@ -2231,7 +2248,7 @@ FFWD_B200_API ffwd_b200_late_ctx_t *ffwd_b200_late_load(const char *model_dir) {
         fail("late load %s: missing linear.weight", model_dir);
         return nullptr;
     }
-    ffwd_b200_ctx *base = load_ctx(model_dir);
+    ffwd_b200_ctx *base = load_ctx(model_dir, linear_i8);
     if (!base) return nullptr;
     const int H = base->cfg.hidden_size;
     std::vector<float> w;
@@ -2257,6 +2274,23 @@ FFWD_B200_API ffwd_b200_late_ctx_t *ffwd_b200_late_load(const char *model_dir) {
     auto *ctx = new ffwd_b200_late_ctx();
     ctx->base = base;
     return ctx;
+}
+
+}  // namespace
+}  // namespace fb
+
+extern "C" {
+
+FFWD_B200_API ffwd_b200_late_ctx_t *ffwd_b200_late_load(const char *model_dir) {
+    return ffwd_b200_late_load_linear(model_dir, -1);
+}
+
+FFWD_B200_API ffwd_b200_late_ctx_t *ffwd_b200_late_load_linear(const char *model_dir,
+                                                               int linear_i8) {
+    t_err.clear();
+    bool i8 = false;
+    if (!model_dir || !linear_choice(linear_i8, &i8)) return nullptr;
+    return load_late(model_dir, i8);
 }
 
 FFWD_B200_API void ffwd_b200_late_free(ffwd_b200_late_ctx_t *ctx) {

@@ -81,6 +81,7 @@ ABI = {
     "ffwd_b200_set_weights_default": (ctypes.c_int, []),
     "ffwd_b200_set_linear_i8": (ctypes.c_int, [ctypes.c_int]),
     "ffwd_b200_load": (ctypes.c_void_p, [ctypes.c_char_p]),
+    "ffwd_b200_load_linear": (ctypes.c_void_p, [ctypes.c_char_p, ctypes.c_int]),
     "ffwd_b200_free": (None, [ctypes.c_void_p]),
     "ffwd_b200_config": (ctypes.POINTER(ffwd_config_t), [ctypes.c_void_p]),
     "ffwd_b200_encode_into": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
@@ -138,6 +139,7 @@ ABI = {
                                                  ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                                  ctypes.c_void_p]),
     "ffwd_b200_late_load": (ctypes.c_void_p, [ctypes.c_char_p]),
+    "ffwd_b200_late_load_linear": (ctypes.c_void_p, [ctypes.c_char_p, ctypes.c_int]),
     "ffwd_b200_late_free": (None, [ctypes.c_void_p]),
     "ffwd_b200_late_config": (ctypes.POINTER(ffwd_config_t), [ctypes.c_void_p]),
     "ffwd_b200_late_token_dim": (ctypes.c_int, [ctypes.c_void_p]),
@@ -242,12 +244,17 @@ def set_fast_gemm(mode: str) -> int:
     return lib().ffwd_b200_set_fast_gemm(mode.encode())
 
 
+def _linear_choice(linear_i8: bool | None) -> int:
+    return -1 if linear_i8 is None else int(bool(linear_i8))
+
+
 class B200Model:
-    """One loaded model (the reference's ffwd_cuda_ctx_t)."""
+    """One loaded model (the reference's ffwd_cuda_ctx_t).  linear_i8: whether its
+    projections run in 8-bit integers (None: as ffwd_b200_set_linear_i8 says)."""
 
     def __init__(self, model_dir: str, gemm_mode: str | None = None,
                  weight_dtype: str | None = None, devices=None, max_tokens: int | None = None,
-                 linear_i8: bool = False):
+                 linear_i8: bool | None = None):
         L = lib()
         if gemm_mode is not None and L.ffwd_b200_set_fast_gemm(gemm_mode.encode()) != 0:
             raise FfwdError("--gpu-gemm-mode must be f32, tf32, bf16, or 16f")
@@ -269,9 +276,7 @@ class B200Model:
         if max_tokens is not None:
             L.ffwd_b200_set_max_tokens(int(max_tokens))
         self._l = L
-        L.ffwd_b200_set_linear_i8(int(linear_i8))
-        self.h = L.ffwd_b200_load(model_dir.encode())
-        L.ffwd_b200_set_linear_i8(0)
+        self.h = L.ffwd_b200_load_linear(model_dir.encode(), _linear_choice(linear_i8))
         if not self.h:
             raise FfwdError(f"failed to load model: {last_error()}")
         self.config = L.ffwd_b200_config(self.h).contents
@@ -384,14 +389,16 @@ def rerank_input(query, query_n_keep, docs, keeps):
 
 
 class B200Late:
-    """A late-interaction model (the reference's ffwd_cuda_late_ctx_t)."""
+    """A late-interaction model (the reference's ffwd_cuda_late_ctx_t).  linear_i8
+    as in B200Model."""
 
-    def __init__(self, model_dir: str, gemm_mode: str | None = None):
+    def __init__(self, model_dir: str, gemm_mode: str | None = None,
+                 linear_i8: bool | None = None):
         L = lib()
         if gemm_mode is not None and L.ffwd_b200_set_fast_gemm(gemm_mode.encode()) != 0:
             raise FfwdError("--gpu-gemm-mode must be f32, tf32, bf16, or 16f")
         self._l = L
-        self.h = L.ffwd_b200_late_load(model_dir.encode())
+        self.h = L.ffwd_b200_late_load_linear(model_dir.encode(), _linear_choice(linear_i8))
         if not self.h:
             raise FfwdError(f"failed to load late model: {last_error()}")
         self.config = L.ffwd_b200_late_config(self.h).contents

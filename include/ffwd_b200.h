@@ -133,8 +133,9 @@ FFWD_B200_API int ffwd_b200_set_weights_f16(int on);
  * process). */
 FFWD_B200_API int ffwd_b200_set_weights_default(void);
 
-/* No reference counterpart.  With on = 1, the next loads run every projection of
- * a layer in 8-bit integers (weights quantised with a scale per output channel
+/* No reference counterpart.  With on = 1, the next loads that make no choice of
+ * their own (ffwd_b200_load_linear) run every projection of a layer in 8-bit
+ * integers (weights quantised with a scale per output channel
  * as they are uploaded, activations with a scale per token as they are
  * produced; exact 32-bit sums), with the plan's 16-bit attention and f32
  * residual stream, norms and embedding: ffwd_b200_precision 5.  Goes with a
@@ -144,6 +145,10 @@ FFWD_B200_API int ffwd_b200_set_linear_i8(int on);
 /* Load config + safetensors from model_dir and upload to every device of the
  * current device set.  Replaces ffwd_cuda_load (cuda.h:26; cuda.cu:4306). */
 FFWD_B200_API ffwd_b200_ctx_t *ffwd_b200_load(const char *model_dir);
+/* The same with the projections chosen for this load alone: linear_i8 1 8-bit, 0
+ * not, -1 as ffwd_b200_set_linear_i8 says.  Loads of several threads do not meet
+ * in the process's switch this way. */
+FFWD_B200_API ffwd_b200_ctx_t *ffwd_b200_load_linear(const char *model_dir, int linear_i8);
 /* Replaces ffwd_cuda_free (cuda.h:27). */
 FFWD_B200_API void ffwd_b200_free(ffwd_b200_ctx_t *ctx);
 /* Replaces ffwd_cuda_config (cuda.h:56). */
@@ -177,6 +182,9 @@ typedef struct ffwd_b200_late_ctx ffwd_b200_late_ctx_t;
  * of the device set.  NULL without a 1_Dense head or with a bad projection.
  * Replaces ffwd_cuda_late_load (cuda.h:35; cuda.cu:5267-5296). */
 FFWD_B200_API ffwd_b200_late_ctx_t *ffwd_b200_late_load(const char *model_dir);
+/* The same with the projections chosen as in ffwd_b200_load_linear. */
+FFWD_B200_API ffwd_b200_late_ctx_t *ffwd_b200_late_load_linear(const char *model_dir,
+                                                               int linear_i8);
 /* Replaces ffwd_cuda_late_free (cuda.h:36). */
 FFWD_B200_API void ffwd_b200_late_free(ffwd_b200_late_ctx_t *ctx);
 /* Replaces ffwd_cuda_late_config (cuda.h:37). */
