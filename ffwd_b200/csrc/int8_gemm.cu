@@ -624,8 +624,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Cfg<BN, EPI, HD>::T
         float *norms = reinterpret_cast<float *>(smem + CF::OFF_NORMS);
         if (EPI == kI8Heads) {
             for (int i = et; i < HD; i += 128 * GROUPS) {
-                norms[i] = p.q_norm ? __ldg(p.q_norm + i) : 1.0f;
-                norms[HD + i] = p.k_norm ? __ldg(p.k_norm + i) : 1.0f;
+                norms[i] = p.q_norm ? ld_global(p.q_norm + i) : 1.0f;
+                norms[HD + i] = p.k_norm ? ld_global(p.k_norm + i) : 1.0f;
             }
         }
         // A tile's row scale, column scales and biases are fetched one tile
@@ -634,7 +634,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Cfg<BN, EPI, HD>::T
         float s_next = 0.0f, c_next[LOADS];
         auto fetch = [&](int mb, int nb) {
             const int grow = mb * 2 * BM + (int)rank * BM + row;
-            s_next = grow < p.M ? __ldg(p.xs + grow) : 0.0f;
+            s_next = grow < p.M ? ld_global(p.xs + grow) : 0.0f;
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 const int e = gt + i * 128;
@@ -644,7 +644,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Cfg<BN, EPI, HD>::T
                 const bool second = EPI == kI8Gated && c >= TN;
                 const int col = nb * TN + (second ? c - TN : c);
                 const float *src = e < NC ? (second ? p.ws2 : p.ws) : (second ? p.bias2 : p.bias);
-                if (src && c < BN && col < p.N) c_next[i] = __ldg(src + col);
+                if (src && c < BN && col < p.N) c_next[i] = ld_global(src + col);
             }
         };
         auto keep = [&](float *cols) {
@@ -671,22 +671,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Cfg<BN, EPI, HD>::T
             if constexpr (EPI == kI8Heads) {
                 if (mb0 != rope_mb) {
                     // The rotary rows of this row block: a warp copies 16 rows,
-                    // one at a time.  All warps are past their last reads.
+                    // eight loads before their stores (32768 x 4096 x 1024 heads
+                    // 153 us, one at a time 168).  All warps are past their last reads.
                     rope_mb = mb0;
                     named_bar(1 + GROUPS, 128 * GROUPS);
-                    const int ps = grow < p.M ? __ldg(p.pos + grow) : 0;
+                    const int ps = grow < p.M ? ld_global(p.pos + grow) : 0;
                     bad = ps < 0 || ps >= p.n_pos;
                     if (bad) set_error(p.err, kErrBadPosition);
                     constexpr int V = HD / 4;  // float4 per row, cos then sin
-#pragma unroll 8
-                    for (int i = 0; i < 16; ++i) {
-                        const int r = q * 32 + g * 16 + i;
-                        int rp = __shfl_sync(0xffffffffu, ps, g * 16 + i);
-                        if (rp < 0 || rp >= p.n_pos) rp = 0;
+#pragma unroll
+                    for (int i0 = 0; i0 < 16; i0 += 8) {
+                        float4 v[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            int rp = __shfl_sync(0xffffffffu, ps, g * 16 + i0 + i);
+                            if (rp < 0 || rp >= p.n_pos) rp = 0;
+                            const float *src =
+                                (lane % V < V / 2 ? p.cos : p.sin) + (size_t)rp * (HD / 2);
+                            v[i] = ld_global(reinterpret_cast<const float4 *>(src) + lane % (V / 2));
+                        }
                         if (lane < V) {
-                            const float *src = (lane < V / 2 ? p.cos : p.sin) + (size_t)rp * (HD / 2);
-                            reinterpret_cast<float4 *>(rope + r * CF::ROPE_LD)[lane] =
-                                __ldg(reinterpret_cast<const float4 *>(src) + lane % (V / 2));
+                            const int r = q * 32 + g * 16 + i0;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                reinterpret_cast<float4 *>(rope + (r + i) * CF::ROPE_LD)[lane] = v[i];
                         }
                     }
                     named_bar(1 + GROUPS, 128 * GROUPS);

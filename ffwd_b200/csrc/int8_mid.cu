@@ -219,12 +219,12 @@ __global__ void __launch_bounds__(kThreads)
         const int per = T / split, t0 = rank * per;
         const int col = c0 + n;
         const bool in = col < p.N;
-        const float ws = in ? __ldg(p.ws + col) : 0.0f;
-        const float b = in && p.bias ? __ldg(p.bias + col) : 0.0f;
+        const float ws = in ? ld_global(p.ws + col) : 0.0f;
+        const float b = in && p.bias ? ld_global(p.bias + col) : 0.0f;
         float ws2 = 0.0f, b2 = 0.0f;
         if (EPI == kI8Gated && in) {
-            ws2 = __ldg(p.ws2 + col);
-            if (p.bias2) b2 = __ldg(p.bias2 + col);
+            ws2 = ld_global(p.ws2 + col);
+            if (p.bias2) b2 = ld_global(p.bias2 + col);
         }
         // Rows [t, t + kRows) of the sums m, over the cluster: all loads of a CTA's
         // sums in flight at once.
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kThreads)
         };
         auto scales8 = [&](int t, float(&s)[kRows]) {
 #pragma unroll
-            for (int i = 0; i < kRows; ++i) s[i] = t + i < t1 ? __ldg(p.xs + row0 + t + i) : 0.0f;
+            for (int i = 0; i < kRows; ++i) s[i] = t + i < t1 ? ld_global(p.xs + row0 + t + i) : 0.0f;
         };
         auto store8 = [&](int t, const float(&y)[kRows]) {
             if (!in) return;
@@ -300,8 +300,8 @@ __global__ void __launch_bounds__(kThreads)
             // The other value of this one's rotation, and its sign.
             const int half = HD / 2, pair = e < half ? n + half : n - half;
             const float sign = e < half ? -1.0f : 1.0f;
-            const float w1 = nw ? __ldg(nw + e) : 1.0f;
-            const float w2 = nw ? __ldg(nw + (e < half ? e + half : e - half)) : 1.0f;
+            const float w1 = nw ? ld_global(nw + e) : 1.0f;
+            const float w2 = nw ? ld_global(nw + (e < half ? e + half : e - half)) : 1.0f;
 #pragma unroll 1
             for (int t = t0 + g * kRows; t < t1; t += 2 * kRows) {
                 float s[kRows], y[kRows], cs[kRows], sn[kRows];
@@ -309,12 +309,12 @@ __global__ void __launch_bounds__(kThreads)
                 uint32_t bad = 0;
 #pragma unroll
                 for (int i = 0; i < kRows; ++i) {
-                    const int ps = rot && t + i < t1 ? __ldg(p.pos + row0 + t + i) : 0;
+                    const int ps = rot && t + i < t1 ? ld_global(p.pos + row0 + t + i) : 0;
                     const bool out = ps < 0 || ps >= p.n_pos;
                     bad |= (uint32_t)out << i;
                     const size_t at = (size_t)(out ? 0 : ps) * half + e % half;
-                    cs[i] = __ldg(p.cos + at);
-                    sn[i] = __ldg(p.sin + at);
+                    cs[i] = ld_global(p.cos + at);
+                    sn[i] = ld_global(p.sin + at);
                 }
                 if (bad && in) set_error(p.err, kErrBadPosition);
                 values8(0, t, ws, b, s, y);

@@ -49,7 +49,7 @@ struct Raw {
             if (TYPE == kI8F32) {
                 const uint32_t *p = static_cast<const uint32_t *>(x) + off + ch;
                 if (COVER != kScalar) {
-                    const uint4 r = __ldg(reinterpret_cast<const uint4 *>(p));
+                    const uint4 r = ld_global(reinterpret_cast<const uint4 *>(p));
                     w[4 * h] = r.x;
                     w[4 * h + 1] = r.y;
                     w[4 * h + 2] = r.z;
@@ -61,7 +61,7 @@ struct Raw {
             } else {
                 const uint16_t *p = static_cast<const uint16_t *>(x) + off + ch;
                 if (COVER != kScalar) {
-                    const uint2 r = __ldg(reinterpret_cast<const uint2 *>(p));
+                    const uint2 r = ld_global(reinterpret_cast<const uint2 *>(p));
                     w[2 * h] = r.x;
                     w[2 * h + 1] = r.y;
                 } else {

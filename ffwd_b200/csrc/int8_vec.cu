@@ -20,7 +20,7 @@ namespace {
 
 
 __device__ __forceinline__ uint4 ldg16(const int8_t *p) {
-    return __ldg(reinterpret_cast<const uint4 *>(p));
+    return ld_global(reinterpret_cast<const uint4 *>(p));
 }
 
 // Bytes of chunk [k, k + 16) at or past K cleared (weights and rows may hold
@@ -104,7 +104,7 @@ __device__ __forceinline__ int mine(const int (&acc)[R][MT], int lane) {
 
 __device__ __forceinline__ float scaled(int acc, float s, const float *ws, const float *bias,
                                         int n) {
-    return fmaf((float)acc * s, __ldg(ws + n), bias ? __ldg(bias + n) : 0.0f);
+    return fmaf((float)acc * s, ld_global(ws + n), bias ? ld_global(bias + n) : 0.0f);
 }
 
 // The first 2 KB of a row on their way to L2; before the wait for the stream's
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kWarps * 32) vec_store_kernel(const I8Params p
     const int n = n0 + lane / MT, m = lane % MT;
     if (lane < R * MT && n < p.N && m < p.M)
         i8::store1(p.y, p.type, (size_t)m * p.ldy + n,
-                   i8::act1(scaled(a, __ldg(p.xs + m), p.ws, p.bias, n), p.act), p.accumulate);
+                   i8::act1(scaled(a, ld_global(p.xs + m), p.ws, p.bias, n), p.act), p.accumulate);
 }
 
 // R columns of gate and up each.
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kWarps * 32) vec_gated_kernel(const I8Params p
     const int up = __shfl_down_sync(0xffffffffu, v, R * MT);
     const int n = n0 + lane / MT, m = lane % MT;
     if (lane < R * MT && n < p.N && m < p.M) {
-        const float s = __ldg(p.xs + m);
+        const float s = ld_global(p.xs + m);
         const float g = i8::act1(scaled(v, s, p.ws, p.bias, n), p.act);
         i8::store1(p.y, p.type, (size_t)m * p.ldy + n, g * scaled(up, s, p.ws2, p.bias2, n), 0);
     }
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kHeadWarps * 32) vec_heads_kernel(const I8Para
         const int a = mine<R, MT>(acc, lane);
         const int r = lane / MT, m = lane % MT;
         if (lane < R * MT)
-            v[m][e0 + r] = m < p.M ? scaled(a, __ldg(p.xs + m), p.ws, p.bias, n0 + r) : 0.0f;
+            v[m][e0 + r] = m < p.M ? scaled(a, ld_global(p.xs + m), p.ws, p.bias, n0 + r) : 0.0f;
     }
     __syncthreads();
     const int m = warp;  // one warp per row
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kHeadWarps * 32) vec_heads_kernel(const I8Para
     }
     if (head < p.n_q_heads + p.n_kv_heads) {
         const float *nw = head < p.n_q_heads ? p.q_norm : p.k_norm;
-        const int ps = __ldg(p.pos + m);
+        const int ps = ld_global(p.pos + m);
         const bool bad = ps < 0 || ps >= p.n_pos;
         if (bad && lane == 0) set_error(p.err, kErrBadPosition);
         float inv = bad ? i8::nan_f() : 1.0f;
@@ -218,9 +218,9 @@ __global__ void __launch_bounds__(kHeadWarps * 32) vec_heads_kernel(const I8Para
 #pragma unroll
         for (int j = 0; j < HALF / 32; ++j) {
             const int e = lane + 32 * j;
-            const float c = __ldg(p.cos + t + e), s = __ldg(p.sin + t + e);
-            const float x1 = a[j] * inv * (nw ? __ldg(nw + e) : 1.0f);
-            const float x2 = b[j] * inv * (nw ? __ldg(nw + HALF + e) : 1.0f);
+            const float c = ld_global(p.cos + t + e), s = ld_global(p.sin + t + e);
+            const float x1 = a[j] * inv * (nw ? ld_global(nw + e) : 1.0f);
+            const float x2 = b[j] * inv * (nw ? ld_global(nw + HALF + e) : 1.0f);
             a[j] = x1 * c - x2 * s;
             b[j] = x2 * c + x1 * s;
         }
