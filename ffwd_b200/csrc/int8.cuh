@@ -55,8 +55,8 @@ struct I8Params {
 
 // x [M, K] of `type` (row stride ldx elements) -> q int8 [M, K] (row stride
 // ldq, a multiple of 16) and s [M]; with `norm`, of x * norm / rms(x) instead.
-// A row of zeros has s = 0; a row whose values (or sum of squares) are not
-// finite has s = NaN and q = 0.  Returns a cudaError_t value.
+// A row of zeros has s = 0; a row whose values (or products with norm, or sum of
+// squares) are not finite has s = NaN and q = 0.  Returns a cudaError_t value.
 int i8_quantize_launch(const void *x, int type, long long ldx, const float *norm, float eps,
                        int8_t *q, long long ldq, float *s, int M, int K, int num_sms,
                        cudaStream_t stream);

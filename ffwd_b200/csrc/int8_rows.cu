@@ -9,7 +9,8 @@
 // there it is taken again in f64: about one value in 10^5 of f32 rows, and of
 // bf16 rows one in 450, which lie on a border exactly.  The row's RMS cancels
 // out of v / s, so with `norm` the codes depend on x * norm alone and only the
-// scale carries the RMS.
+// scale carries the RMS.  Rows below 1e-30 (the largest value, or with `norm` the
+// largest product or the mean square) are worked on in f64 throughout.
 #include "int8.cuh"
 #include "launch_util.cuh"
 #include "ptx.cuh"
@@ -197,6 +198,22 @@ __device__ __forceinline__ bool put8(float (&x)[8], const float (&g)[8], float i
     return any;
 }
 
+// Zeros at columns c and c + 128 on.
+template <int COVER>
+__device__ __forceinline__ void zero8(int8_t *q, int c, int K) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int ch = c + 128 * h;
+        if (COVER != kScalar) {
+            if (COVER == kFull || ch < K) *reinterpret_cast<uint32_t *>(q + ch) = 0u;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (ch + i < K) q[ch + i] = 0;
+        }
+    }
+}
+
 // Blocks per SM that the registers allow: the row's values twice (this row's
 // and the next one's, in flight).
 constexpr int min_blocks(int type, bool norm, int w, int nv) {
@@ -215,6 +232,7 @@ __global__ void __launch_bounds__((W == 1 ? 8 : W) * 32, min_blocks(TYPE, NORM, 
     constexpr int NW = W == 1 ? 8 : W, R = NW / W;  // rows of a block at a time
     __shared__ uint32_t sh_max[NW];
     __shared__ float sh_sum[NW], sh_lo[NW];
+    __shared__ double sh_max64[NORM ? NW : 1], sh_sum64[NORM ? NW : 1];
     griddep_wait();
     griddep_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -246,11 +264,15 @@ __global__ void __launch_bounds__((W == 1 ? 8 : W) * 32, min_blocks(TYPE, NORM, 
         auto each = [&](auto f) {
             float v[8], g[8];
             if (NV > 0) {
+                // (the next group's weights on their way while one is worked on)
+                Raw<kI8F32, COVER> w;
+                if (NORM) w.load(norm, 0, c0, K);
 #pragma unroll
                 for (int k = 0; k < NR; ++k) {
                     const int c = k * W * 256 + c0;
                     raw[k].unpack(v);
-                    if (NORM) load_norm<COVER>(norm, c, K, g);
+                    if (NORM) w.unpack(g);
+                    if (NORM && k + 1 < NR) w.load(norm, 0, c + W * 256, K);
                     f(v, g, c);
                 }
             } else {
@@ -305,12 +327,12 @@ __global__ void __launch_bounds__((W == 1 ? 8 : W) * 32, min_blocks(TYPE, NORM, 
         }
         const float amax = __uint_as_float(mx);
         const bool finite = mx < 0x7F800000u && (!NORM || ss < INFINITY);
-        const bool plain = live && finite && amax >= 1e-30f;
+        // (a mean square below 1e-30: the squares may have left f32)
+        const bool plain = live && finite && amax >= 1e-30f &&
+                           (!NORM || fmaf(eps, (float)K, ss) >= 1e-30f * (float)K);
         int8_t *qr = q + (size_t)row * ldq;
-        if (live && t == 0)
-            s[row] = !finite ? __uint_as_float(0x7FC00000u)
-                     : NORM  ? amax / 127.0f / sqrtf(ss / (float)K + eps)
-                             : amax / 127.0f;
+        if (plain && t == 0)
+            s[row] = NORM ? amax / 127.0f / sqrtf(ss / (float)K + eps) : amax / 127.0f;
         const float inv = 127.0f / amax;
         bool open = false;  // codes left to settle
         if (plain)
@@ -318,14 +340,60 @@ __global__ void __launch_bounds__((W == 1 ? 8 : W) * 32, min_blocks(TYPE, NORM, 
                 if (COVER == kFull || c < K) open |= put8<NORM, !NORM, COVER>(a, b, inv, amax, 0.0f, qr, c, K);
             });
         if (live && !plain) {
-            // 127 / amax may pass f32 for rows so small: a value at a time, in
-            // f64.  Rows of zeros, or not finite, get zeros.
+            // 127 / amax may pass f32 for rows so small, and their products with
+            // the weights and their squares may be below it: a value at a time, in
+            // f64 (W > 1: a row is all of the block's, so the block meets here).
+            // Rows of zeros, or not finite, get zeros.
+            double am = finite ? amax : 0.0f, rms = 1.0;
+            bool some = finite;
+            if (NORM && mx == 0) {  // zeros, or products below f32
+                some = false;
+                each([&](const float(&a)[8], const float(&)[8], int) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) some |= a[i] != 0.0f;
+                });
+                some = W == 1 ? __any_sync(0xffffffffu, some) : __syncthreads_or(some);
+            }
+            if (NORM && some) {
+                double sq = 0.0;
+                am = 0.0;
 #pragma unroll 1
-            for (int c = t; c < K; c += W * 32) {
+                for (int c = t; c < K; c += W * 32) {
+                    const double v = (double)load1<TYPE>(x, off + c);
+                    am = fmax(am, fabs(v * (double)norm[c]));
+                    sq = fma(v, v, sq);
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    am = fmax(am, __shfl_xor_sync(0xffffffffu, am, o));
+                    sq += __shfl_xor_sync(0xffffffffu, sq, o);
+                }
+                if (W > 1) {
+                    if (lane == 0) {
+                        sh_max64[warp] = am;
+                        sh_sum64[warp] = sq;
+                    }
+                    __syncthreads();
+                    sq = 0.0;
+#pragma unroll 1
+                    for (int i = 0; i < W; ++i) {
+                        am = fmax(am, sh_max64[i]);
+                        sq += sh_sum64[i];
+                    }
+                }
+                rms = sqrt(sq / (double)K + (double)eps);
+            }
+            const double sc = am / 127.0;
+            if (t == 0) s[row] = finite ? (float)(sc / rms) : __uint_as_float(0x7FC00000u);
+#pragma unroll 1
+            for (int c = t; am > 0.0 && c < K; c += W * 32) {
                 double v = (double)load1<TYPE>(x, off + c);
                 if (NORM) v *= (double)norm[c];
-                qr[c] = finite && amax > 0.0f ? (int8_t)(int)rint(v / ((double)amax / 127.0)) : 0;
+                qr[c] = (int8_t)(int)rint(v / sc);
             }
+            if (!(am > 0.0))
+#pragma unroll 1
+                for (int c = c0; c < K; c += W * 256) zero8<COVER>(qr, c, K);
         }
         if (NORM) {
             // Settling takes the largest product in full: among the values whose

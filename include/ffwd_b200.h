@@ -403,8 +403,8 @@ typedef struct {
 /* x [M, K] of `type` (row stride ldx elements) -> q int8 [M, K] (16-byte
  * aligned, row stride ldq a multiple of 16; bytes past K are left alone) and
  * scale [M].  With `norm` [K], of x * norm / sqrt(mean(x^2) + eps) instead.
- * A row of zeros gets scale 0; a row with a value (or, with `norm`, a sum of
- * squares) that is not finite gets scale NaN and zeros.  Also quantises
+ * A row of zeros gets scale 0; a row with a value (or, with `norm`, a product or
+ * the sum of squares in f32) that is not finite gets scale NaN and zeros.  Also quantises
  * weights: a row per output channel. */
 FFWD_B200_API int ffwd_b200_quantize_i8(const void *x, int type, long long ldx, const float *norm,
                                         float eps, int8_t *q, long long ldq, float *scale, int M,
