@@ -1214,6 +1214,8 @@ int check_err(Device &D) {
              e == kErrBadTokenId ? "invalid token id"
              : e == kErrBadNorm  ? "zero or non-finite embedding norm"
              : e == kErrWaitTimeout ? "device wait timed out"
+             : e == kErrSmemAlign   ? "shared memory window not aligned"
+             : e == kErrBadPosition ? "position outside the rotary tables"
                                     : "unknown");
         return -1;
     }

@@ -18,3 +18,15 @@ def test_no_read_only_loads():
     for path in files:
         text = open(path).read()
         assert not re.search(r"__ldg|__ldcs|ld\.global[.\w]*\.nc|__restrict__", text), path
+
+
+def test_every_device_error_has_a_text():
+    """The host names each code that a kernel can record."""
+    enum = re.search(r"enum DevError : int \{(.*?)\};", open(os.path.join(CSRC, "ptx.cuh")).read(),
+                     re.S).group(1)
+    codes = [c for c in re.findall(r"\b(kErr\w+) =", enum) if c != "kErrNone"]
+    assert "kErrBadPosition" in codes
+    engine = open(os.path.join(CSRC, "engine.cu")).read()
+    text = engine[engine.index("int check_err(Device &D) {"):]
+    text = text[:text.index("\n}\n")]
+    assert [c for c in codes if c not in text] == []
