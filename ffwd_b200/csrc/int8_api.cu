@@ -35,9 +35,10 @@ constexpr int kMaxRows = 1 << 30;
 
 bool type_ok(int t) { return t == kI8F32 || t == kI8BF16 || t == kI8F16; }
 
-// Shapes, strides and alignment of the quantised rows.
+// Shapes, strides and alignment of the quantised rows.  (No rows: a tensor
+// without elements has no address.)
 int check_rows(const int8_t *x, long long ldx, const float *xs, int M, int K) {
-    if (M < 0 || M > kMaxRows || !x || !xs) {
+    if (M < 0 || M > kMaxRows || (M > 0 && (!x || !xs))) {
         fail("invalid arguments");
         return -1;
     }
@@ -76,8 +77,8 @@ int check_mat(const ffwd_b200_i8_mat_t *w) {
     return 0;
 }
 
-int check_out(const void *y, int type, long long ldy, int N) {
-    if (!y || !type_ok(type)) {
+int check_out(const void *y, int type, long long ldy, int M, int N) {
+    if ((M > 0 && !y) || !type_ok(type)) {
         fail("invalid arguments");
         return -1;
     }
@@ -139,7 +140,7 @@ FFWD_B200_API int ffwd_b200_quantize_i8(const void *x, int type, long long ldx, 
                                         float eps, int8_t *q, long long ldq, float *scale, int M,
                                         int K, void *stream) {
     clear_error();
-    if (!x || !q || !scale || !type_ok(type) || M < 0 || M > kMaxRows || K <= 0 ||
+    if ((M > 0 && (!x || !q || !scale)) || !type_ok(type) || M < 0 || M > kMaxRows || K <= 0 ||
         K > kMaxRows) {
         fail("invalid arguments");
         return -1;
@@ -178,7 +179,7 @@ FFWD_B200_API int ffwd_b200_gemm_i8(const ffwd_b200_i8_mat_t *w, const int8_t *x
                                     const float *xs, int M, void *y, int type, long long ldy,
                                     int act, int accumulate, int *err, void *stream) {
     clear_error();
-    if (check_mat(w) || check_rows(x, ldx, xs, M, w->cols) || check_out(y, type, ldy, w->rows))
+    if (check_mat(w) || check_rows(x, ldx, xs, M, w->cols) || check_out(y, type, ldy, M, w->rows))
         return -1;
     if (act < kI8None || act > kI8GeluTanh) {
         fail("unknown activation %d", act);
@@ -213,7 +214,7 @@ FFWD_B200_API int ffwd_b200_gated_i8(const ffwd_b200_i8_mat_t *gate, const ffwd_
         fail("gate is %d x %d, up %d x %d", gate->rows, gate->cols, up->rows, up->cols);
         return -1;
     }
-    if (check_rows(x, ldx, xs, M, gate->cols) || check_out(h, type, ldh, gate->rows)) return -1;
+    if (check_rows(x, ldx, xs, M, gate->cols) || check_out(h, type, ldh, M, gate->rows)) return -1;
     if (act < kI8Silu || act > kI8GeluTanh) {
         fail("unknown gate activation %d", act);
         return -1;
@@ -242,7 +243,7 @@ FFWD_B200_API int ffwd_b200_qkv_i8(const ffwd_b200_i8_mat_t *w, const ffwd_b200_
     clear_error();
     if (check_mat(w)) return -1;
     if (!heads || heads->n_heads <= 0 || heads->n_kv_heads <= 0 || heads->n_pos <= 0 ||
-        !heads->pos || !heads->cos || !heads->sin) {
+        (M > 0 && !heads->pos) || !heads->cos || !heads->sin) {
         fail("invalid heads");
         return -1;
     }
@@ -264,7 +265,7 @@ FFWD_B200_API int ffwd_b200_qkv_i8(const ffwd_b200_i8_mat_t *w, const ffwd_b200_
         fail("rotary tables and head norms need 16-byte alignment");
         return -1;
     }
-    if (check_rows(x, ldx, xs, M, w->cols) || check_out(out, type, ldo, w->rows)) return -1;
+    if (check_rows(x, ldx, xs, M, w->cols) || check_out(out, type, ldo, M, w->rows)) return -1;
     I8Params p{};
     p.M = M;
     set_mat(p, w);

@@ -360,8 +360,9 @@ FFWD_B200_API int ffwd_b200_gemm_tf32(const float *x, const float *w, float *y, 
  * Work is enqueued on `stream` (a cudaStream_t of the current device; NULL is
  * the default stream); nothing is allocated, kept or synchronised, so the calls
  * can be captured into CUDA graphs.  Outputs must not overlap inputs.  M = 0
- * is an empty call; a call has at most 2^30 rows, and weights as many channels.  `err` is an int in device memory, zeroed by the caller,
- * or NULL: a kernel that fails records a nonzero code there (1: a device wait
+ * is an empty call (its rows' and outputs' pointers may be NULL); a call has at
+ * most 2^30 rows, and weights as many channels.  `err` is an int in device
+ * memory, zeroed by the caller, or NULL: a kernel that fails records a nonzero code there (1: a device wait
  * ran out, 5: a position outside the rotary tables). */
 enum {
     FFWD_B200_F32 = 0,
