@@ -82,6 +82,12 @@ __device__ __forceinline__ float2 act2(float2 x, int act) {
 
 __device__ __forceinline__ float act1(float x, int act) { return act2(make_float2(x, x), act).x; }
 
+// A value z rotated with its head's other half o: z c -+ o s (- in the first half,
+// where sign is -1), rounded alike in every kernel.
+__device__ __forceinline__ float rotate(float z, float o, float c, float s, float sign) {
+    return fmaf(sign * o, s, __fmul_rn(z, c));
+}
+
 __device__ __forceinline__ float nan_f() { return __uint_as_float(0x7FC00000u); }
 
 __device__ __forceinline__ uint16_t to_16(float v, int type) {

@@ -391,6 +391,7 @@ __device__ __forceinline__ void epilogue_heads(const I8Params &p, uint32_t tbase
                             a = mul_f32x2(a, u ? make_float2(w1.z, w1.w) : make_float2(w1.x, w1.y));
                             b = mul_f32x2(b, u ? make_float2(w2.z, w2.w) : make_float2(w2.x, w2.y));
                         }
+                        // (as i8::rotate)
                         const float2 r1 = mul_f32x2(a, c2);
                         const float2 r2 = fma_f32x2(a, s2, mul_f32x2(b, c2));
                         A[j] = fmaf(-b.x, s2.x, r1.x);

@@ -347,8 +347,8 @@ __global__ void __launch_bounds__(kThreads)
                             for (int k = 0; k < HD / 32; ++k) ss += part[tt * 4 + first + k];
                             inv *= 1.0f / sqrtf(ss / (float)HD + p.eps);
                         }
-                        y[i] = y[i] * inv * w1 * cs[i] +
-                               sign * (values[tt * BC + pair] * inv * w2 * sn[i]);
+                        y[i] = i8::rotate(y[i] * inv * w1, values[tt * BC + pair] * inv * w2, cs[i],
+                                          sn[i], sign);
                     }
                 }
                 store8(t, y);

@@ -221,8 +221,8 @@ __global__ void __launch_bounds__(kHeadWarps * 32) vec_heads_kernel(const I8Para
             const float c = ld_global(p.cos + t + e), s = ld_global(p.sin + t + e);
             const float x1 = a[j] * inv * (nw ? ld_global(nw + e) : 1.0f);
             const float x2 = b[j] * inv * (nw ? ld_global(nw + HALF + e) : 1.0f);
-            a[j] = x1 * c - x2 * s;
-            b[j] = x2 * c + x1 * s;
+            a[j] = i8::rotate(x1, x2, c, s, -1.0f);
+            b[j] = i8::rotate(x2, x1, c, s, 1.0f);
         }
     }
     const size_t o = (size_t)m * p.ldy + (size_t)head * HD;
