@@ -66,7 +66,7 @@ __device__ __forceinline__ float2 silu(float2 x) {
 // GELU, tanh form: 0.5 (1 + tanh(v)) = 1 / (1 + 2^e), v = sqrt(2 / pi) (x +
 // 0.044715 x^3), e = -2 log2(e) v.
 __device__ __forceinline__ float2 gelu_tanh(float2 x) {
-    const float2 k = fma_f32x2(mul_f32x2(x, x), both(-0.1029432f), both(-2.3022082f));
+    const float2 k = fma_f32x2(mul_f32x2(x, x), both(-0.10294324f), both(-2.3022082f));
     const float2 e = mul_f32x2(x, k);
     return over_1p(x, make_float2(ex2_approx(e.x), ex2_approx(e.y)));
 }
