@@ -18,7 +18,6 @@
 namespace fb {
 namespace {
 
-
 __device__ __forceinline__ uint4 ldg16(const int8_t *p) {
     return ld_global(reinterpret_cast<const uint4 *>(p));
 }
@@ -254,9 +253,15 @@ cudaError_t run(int epi, const I8Params &p, int num_sms, cudaStream_t st) {
     switch (epi) {
     case kI8Store:
         if (MT == 4 || p.N >= 4 * warps) return run_store<4, MT>(p, st);
-        return MT == 2 || p.N >= 2 * warps ? run_store<2, MT>(p, st) : run_store<1, MT>(p, st);
+        if constexpr (MT == 1) {
+            if (p.N < 2 * warps) return run_store<1, MT>(p, st);
+        }
+        if constexpr (MT <= 2) return run_store<2, MT>(p, st);
+        break;
     case kI8Gated:
-        return MT == 4 || p.N >= 2 * warps ? run_gated<2, MT>(p, st) : run_gated<1, MT>(p, st);
+        if (MT == 4 || p.N >= 2 * warps) return run_gated<2, MT>(p, st);
+        if constexpr (MT <= 2) return run_gated<1, MT>(p, st);
+        break;
     case kI8Heads: {
         const int heads = p.n_q_heads + 2 * p.n_kv_heads;
         return p.head_dim == 128 ? launch_k(vec_heads_kernel<128, MT>, dim3(heads),

@@ -66,3 +66,20 @@ def test_heads(K, hd, dtype):
             whole = out
         assert torch.equal(out[:, h * hd:], whole[:M, h * hd:]), M
         within(out[:, :h * hd], want[:M, :h * hd], bound[:M, :h * hd])
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 4])
+@pytest.mark.parametrize("N", [100, 4737, 9999])
+@pytest.mark.parametrize("K", [45, 700])
+def test_few_rows_of_every_width(M, N, K):
+    """One, two and four weight rows a warp, their last ones past the matrix."""
+    x, s = rows(M, K, 1)
+    w, t = rows(N, K, 2)
+    u, v = rows(N, K, 3)
+    y = torch.full((M, N), float("nan"), device=DEV)
+    h = y.clone()
+    native.gemm_i8(mat(w, t, K), x.data_ptr(), x.stride(0), s.data_ptr(), M, y.data_ptr(), "f32", N)
+    native.gated_i8(mat(w, t, K), mat(u, v, K), x.data_ptr(), x.stride(0), s.data_ptr(), M,
+                    h.data_ptr(), "f32", N)
+    within(y, *ref.gemm(x[:, :K], s, w[:, :K], t, None, "none", "f32"))
+    within(h, *ref.gated(x[:, :K], s, w[:, :K], t, None, u[:, :K], v, None, "silu", "f32"))
