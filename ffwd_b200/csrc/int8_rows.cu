@@ -264,15 +264,18 @@ __global__ void __launch_bounds__((W == 1 ? 8 : W) * 32, min_blocks(TYPE, NORM, 
         auto each = [&](auto f) {
             float v[8], g[8];
             if (NV > 0) {
-                // (the next group's weights on their way while one is worked on)
+                // (f32 rows: the next group's weights on their way while one is worked
+                // on; rows of 16 bits have no registers for them, 8192 x 4096 f16 31
+                // us without, 34 with spills)
                 Raw<kI8F32, COVER> w;
-                if (NORM) w.load(norm, 0, c0, K);
+                if (NORM && TYPE == kI8F32) w.load(norm, 0, c0, K);
 #pragma unroll
                 for (int k = 0; k < NR; ++k) {
                     const int c = k * W * 256 + c0;
                     raw[k].unpack(v);
+                    if (NORM && TYPE != kI8F32) w.load(norm, 0, c, K);
                     if (NORM) w.unpack(g);
-                    if (NORM && k + 1 < NR) w.load(norm, 0, c + W * 256, K);
+                    if (NORM && TYPE == kI8F32 && k + 1 < NR) w.load(norm, 0, c + W * 256, K);
                     f(v, g, c);
                 }
             } else {
