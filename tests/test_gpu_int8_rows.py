@@ -21,6 +21,7 @@ def check(q, s, x, norm, eps, terms):
     where the scale is below its normal range."""
     qe, se = ref.quantise(x, norm, torch.tensor(eps, dtype=torch.float32).item())
     assert torch.equal(q[:, :x.shape[1]], qe)
+    assert (q[:, x.shape[1]:] == 99).all()  # padding left alone
     n = 4 + terms / 2
     assert ((s.double() - se).abs() <= n * ref.U * se + 2.0 ** -150).all()
 
